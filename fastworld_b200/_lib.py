@@ -15,6 +15,8 @@ FW_MAX_ACTION_BLOCKS = 64
 FW_MAX_STEPS = 16
 KIND_WEIGHT, KIND_STATE, KIND_INPUT, KIND_OUTPUT, KIND_WORKSPACE, KIND_STATUS, KIND_DERIVED = range(7)
 DT_BF16, DT_F32, DT_I32, DT_U8, DT_F16 = range(5)
+NORM_NONE, NORM_LAYER, NORM_RMS = range(3)
+BLOCK_MAX_COLS, NORM_MAX_COLS = 1 << 24, 16384
 EPI_BF16, EPI_GELU_BF16, EPI_RESID_F32, EPI_F32, EPI_GELU_ERF_BF16 = range(5)
 
 
@@ -48,6 +50,15 @@ class FwPrepArgs(ctypes.Structure):
     _fields_ = [("chunk", ctypes.c_int), ("seed", ctypes.c_ulonglong), ("draw_noise", ctypes.c_int),
                 ("cond", ctypes.c_void_p), ("cond_frames", ctypes.c_int), ("j_lo", ctypes.c_int),
                 ("n_act", ctypes.c_int), ("actions", ctypes.c_float * (FW_PREP_MAX_ACT * 8))]
+
+
+class FwNormArgs(ctypes.Structure):
+    _fields_ = [("resid", ctypes.c_void_p), ("y", ctypes.c_void_p), ("y_dtype", ctypes.c_int), ("post", ctypes.c_int),
+                ("pre", ctypes.c_int), ("post_w", ctypes.c_void_p), ("post_b", ctypes.c_void_p),
+                ("pre_w", ctypes.c_void_p), ("pre_b", ctypes.c_void_p), ("gate", ctypes.c_void_p),
+                ("shift", ctypes.c_void_p), ("scale", ctypes.c_void_p), ("resid_scale", ctypes.c_float),
+                ("branch_scale", ctypes.c_float), ("eps", ctypes.c_float), ("M", ctypes.c_int), ("D", ctypes.c_int),
+                ("rows_per_frame", ctypes.c_int), ("out", ctypes.c_void_p), ("out_s", ctypes.c_void_p)]
 
 
 class FwTaehvConfig(ctypes.Structure):
@@ -91,6 +102,12 @@ _SIGS = {
                                     ctypes.c_void_p]),
     "fw_quant_e4m3": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p,
                                      ctypes.c_void_p]),
+    "fw_quant_e4m3_block": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+                                           ctypes.c_void_p, ctypes.c_void_p]),
+    "fw_gemm_e4m3_block": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                                          ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int,
+                                          ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p]),
+    "fw_norm_gate_resid": (ctypes.c_int, [ctypes.POINTER(FwNormArgs), ctypes.c_void_p]),
     "fw_ipc_get_handle": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_char_p, ctypes.POINTER(ctypes.c_size_t)]),
     "fw_ipc_open": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(ctypes.c_void_p)]),
     "fw_ipc_close": (ctypes.c_int, [ctypes.c_void_p]),

@@ -1,0 +1,327 @@
+// Row kernels of the block-scaled e4m3 linears (format: fw_block8.cuh): the quantiser, and the norms
+// around a block fused with its gate and residual update.  Both move each byte once; HBM bounds them.
+#include "../../include/fastworld_b200.h"
+#include "fw_block8.cuh"
+#include "fw_internal.h"
+
+namespace fw {
+
+namespace {
+
+// Four consecutive elements as fp32; VEC: the address is aligned to four elements and all are there.
+template <typename T> struct Load4;
+template <> struct Load4<float> {
+  static __device__ __forceinline__ void vec(const float* p, float (&v)[4]) {
+    const float4 u = *reinterpret_cast<const float4*>(p);
+    v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
+  }
+  static __device__ __forceinline__ float one(float x) { return x; }
+};
+template <> struct Load4<__nv_bfloat16> {
+  static __device__ __forceinline__ void vec(const __nv_bfloat16* p, float (&v)[4]) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    const float2 a = unpack_bf16(u.x), b = unpack_bf16(u.y);
+    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+  }
+  static __device__ __forceinline__ float one(__nv_bfloat16 x) { return __bfloat162float(x); }
+};
+template <> struct Load4<__half> {
+  static __device__ __forceinline__ void vec(const __half* p, float (&v)[4]) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
+    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+  }
+  static __device__ __forceinline__ float one(__half x) { return __half2float(x); }
+};
+// Columns [c, c + 4) of a row of K, zeros behind K.
+template <bool VEC, typename T>
+__device__ __forceinline__ void load4(const T* row, int c, int K, float (&v)[4]) {
+  if (VEC) {
+    if (c < K) {
+      Load4<T>::vec(row + c, v);
+    } else {
+      v[0] = v[1] = v[2] = v[3] = 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = c + i < K ? Load4<T>::one(row[c + i]) : 0.f;
+  }
+}
+
+// ---------------------------------------------------------------- quantiser
+// A warp takes one row's group of 512 columns: four blocks, four columns per lane and block, so
+// each load and each store of codes is contiguous over the warp and a block's maximum is one warp
+// reduction.  The eight warps of a CTA take eight neighbouring rows of one group, whose words of exponents are
+// one 32-byte sector.
+constexpr int QROWS = 8;
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(QROWS * 32) quant_block_kernel(const T* __restrict__ x, int M, int K,
+                                                                 uint8_t* __restrict__ q, uint32_t* __restrict__ s) {
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int g = blockIdx.y;
+  const long long row = (long long)blockIdx.x * QROWS + (threadIdx.x >> 5);
+  if (row >= M) return;
+  const int Kp = b8::padded(K), c0 = g * b8::GRP * b8::BLK + lane * 4;
+  const T* src = x + (size_t)row * K;
+  float v[b8::GRP][4];
+#pragma unroll
+  for (int b = 0; b < b8::GRP; ++b) load4<VEC>(src, c0 + b * b8::BLK, K, v[b]);
+  uint32_t word = b8::ONES;
+#pragma unroll
+  for (int b = 0; b < b8::GRP; ++b) {
+    const int c = c0 + b * b8::BLK;
+    if (c < Kp) {   // the same for the whole warp: Kp is a multiple of 128
+      uint32_t eb;
+      const uint32_t code = b8::encode_block(v[b], eb);
+      *reinterpret_cast<uint32_t*>(q + (size_t)row * Kp + c) = code;
+      word = (word & ~(0xffu << (8 * b))) | (eb << (8 * b));
+    }
+  }
+  if (lane == 0) s[(size_t)g * M + row] = word;
+}
+
+template <typename T>
+int quant_launch(const void* x, int M, int K, void* q, void* s, cudaStream_t st) {
+  const dim3 grid((M + QROWS - 1) / QROWS, b8::groups(K));
+  const bool vec = K % 4 == 0 && reinterpret_cast<uintptr_t>(x) % (4 * sizeof(T)) == 0;
+  const cudaError_t e =
+      vec ? launch_k(quant_block_kernel<T, true>, grid, QROWS * 32, 0, st, static_cast<const T*>(x), M, K,
+                     static_cast<uint8_t*>(q), static_cast<uint32_t*>(s))
+          : launch_k(quant_block_kernel<T, false>, grid, QROWS * 32, 0, st, static_cast<const T*>(x), M, K,
+                     static_cast<uint8_t*>(q), static_cast<uint32_t*>(s));
+  return e == cudaSuccess ? FW_OK : FW_ECUDA;
+}
+
+// ---------------------------------------------------------------- norms around a block
+struct NormArgs {
+  float* resid;
+  const void* y;                                  // the block's output, null: no residual update
+  const __nv_bfloat16 *post_w, *post_b, *pre_w, *pre_b;
+  const float *gate, *shift, *scale;              // [frames, D]
+  float resid_scale, branch_scale, eps;
+  int post, pre;                                  // FW_NORM_*
+  int M, D, rows_per_frame;
+  void* out;                                      // bf16 [M, D] or codes [M, Dp]; null: no second norm
+  uint8_t* out_s;                                 // exponents of codes, null: bf16
+};
+
+// One row per CTA of W warps; warp w holds blocks [w NB, w NB + NB) of 128 columns in
+// registers, four columns per lane and block.
+template <int W>
+__device__ __forceinline__ float row_sum(float v, float* slot, int warp, int lane) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (W == 1) return v;
+  if (lane == 0) slot[warp] = v;
+  __syncthreads();
+  float t = 0.f;
+#pragma unroll
+  for (int i = 0; i < W; ++i) t += slot[i];
+  return t;
+}
+
+// Normalises x in place: fp32 mean and, about it, fp32 mean square (two sums, no cancellation).
+template <int W, int NB>
+__device__ __forceinline__ void norm_row(float (&x)[NB][4], int kind, float eps, int D, int c0, float* slots, int warp,
+                                         int lane) {
+  const float inv_d = 1.f / (float)D;
+  if (kind == FW_NORM_LAYER) {
+    float t = 0.f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) t += (x[b][0] + x[b][1]) + (x[b][2] + x[b][3]);   // zeros behind D
+    const float mu = row_sum<W>(t, slots, warp, lane) * inv_d;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[b][i] = c0 + b * b8::BLK + i < D ? x[b][i] - mu : 0.f;
+  }
+  float t = 0.f;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+    t += (x[b][0] * x[b][0] + x[b][1] * x[b][1]) + (x[b][2] * x[b][2] + x[b][3] * x[b][3]);
+  const float r = rsqrtf(row_sum<W>(t, slots + W, warp, lane) * inv_d + eps);
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[b][i] *= r;
+}
+
+template <typename Y, bool VEC, int W, int NB>
+__global__ void __launch_bounds__(W * 32) norm_gate_resid_kernel(const NormArgs a) {
+  pdl_trigger();
+  pdl_wait();
+  __shared__ float slots[4 * W];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row = blockIdx.x, D = a.D;
+  const int b0 = warp * NB, c0 = b0 * b8::BLK + lane * 4;
+  const size_t frame = (size_t)(row / a.rows_per_frame) * D;
+  float* xr = a.resid + (size_t)row * D;
+  float x[NB][4];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) load4<VEC>(xr, c0 + b * b8::BLK, D, x[b]);
+  if (a.y) {
+    float y[NB][4];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) load4<VEC>(static_cast<const Y*>(a.y) + (size_t)row * D, c0 + b * b8::BLK, D, y[b]);
+    if (a.post != FW_NORM_NONE) norm_row<W, NB>(y, a.post, a.eps, D, c0, slots, warp, lane);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const int c = c0 + b * b8::BLK;
+      float p[4];
+      if (a.post_w) {
+        load4<VEC>(a.post_w, c, D, p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[b][i] *= p[i];
+      }
+      if (a.post_b) {
+        load4<VEC>(a.post_b, c, D, p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[b][i] += p[i];
+      }
+      if (a.gate) {
+        load4<VEC>(a.gate + frame, c, D, p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[b][i] *= p[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[b][i] = a.resid_scale * x[b][i] + a.branch_scale * y[b][i];
+      if (VEC) {
+        if (c < D) *reinterpret_cast<float4*>(xr + c) = make_float4(x[b][0], x[b][1], x[b][2], x[b][3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (c + i < D) xr[c + i] = x[b][i];
+      }
+    }
+  }
+  if (!a.out) return;
+  if (a.pre != FW_NORM_NONE) norm_row<W, NB>(x, a.pre, a.eps, D, c0, slots + 2 * W, warp, lane);
+  const int Dp = b8::padded(D);
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const int c = c0 + b * b8::BLK;
+    float p[4];
+    if (a.pre_w) {
+      load4<VEC>(a.pre_w, c, D, p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[b][i] *= p[i];
+    }
+    if (a.pre_b) {
+      load4<VEC>(a.pre_b, c, D, p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[b][i] += p[i];
+    }
+    if (a.scale) {
+      load4<VEC>(a.scale + frame, c, D, p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[b][i] *= 1.f + p[i];
+      load4<VEC>(a.shift + frame, c, D, p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[b][i] += p[i];
+    }
+    if (a.out_s) {
+      const int blk = b0 + b;
+      if (blk * b8::BLK < Dp) {   // zeros behind D: every parameter reads as zero there
+        uint32_t eb;
+        const uint32_t code = b8::encode_block(x[b], eb);
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.out) + (size_t)row * Dp + c) = code;
+        if (lane == 0) a.out_s[((size_t)(blk / b8::GRP) * a.M + row) * b8::GRP + blk % b8::GRP] = (uint8_t)eb;
+      }
+    } else if (VEC) {
+      if (c < D)
+        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + (size_t)row * D + c) =
+            make_uint2(pack_bf16(x[b][0], x[b][1]), pack_bf16(x[b][2], x[b][3]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c + i < D) static_cast<__nv_bfloat16*>(a.out)[(size_t)row * D + c + i] = __float2bfloat16_rn(x[b][i]);
+    }
+  }
+  if (a.out_s && threadIdx.x == 0)   // places behind the last block
+    for (int blk = b8::blocks(D); blk < b8::groups(D) * b8::GRP; ++blk)
+      a.out_s[((size_t)(blk / b8::GRP) * a.M + row) * b8::GRP + blk % b8::GRP] = 127;
+}
+
+template <typename Y, bool VEC>
+int norm_launch(const NormArgs& a, cudaStream_t s) {
+  const int nb = b8::blocks(a.D);
+  auto go = [&](auto kern, int warps) {
+    return launch_k(kern, dim3(a.M), dim3(warps * 32), 0, s, a) == cudaSuccess ? FW_OK : FW_ECUDA;
+  };
+  if (nb <= 4) return go(norm_gate_resid_kernel<Y, VEC, 4, 1>, 4);
+  if (nb <= 12) return go(norm_gate_resid_kernel<Y, VEC, 4, 3>, 4);
+  if (nb <= 48) return go(norm_gate_resid_kernel<Y, VEC, 8, 6>, 8);
+  return go(norm_gate_resid_kernel<Y, VEC, 16, 8>, 16);
+}
+
+}  // namespace
+}  // namespace fw
+
+extern "C" {
+
+int fw_quant_e4m3_block(const void* x, int dtype, int M, int K, void* q, void* s, void* stream) {
+  using namespace fw;
+  if (M < 0 || K <= 0 || K > FW_BLOCK_MAX_COLS) return FW_ESHAPE;
+  if (M == 0) return FW_OK;
+  if (!x || !q || !s) return FW_EINVAL;
+  if (dtype != FW_BF16 && dtype != FW_F16 && dtype != FW_F32) return FW_EINVAL;
+  if (reinterpret_cast<uintptr_t>(q) % 16 || reinterpret_cast<uintptr_t>(s) % 4 ||
+      reinterpret_cast<uintptr_t>(x) % (dtype == FW_F32 ? 4 : 2))
+    return FW_EALIGN;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case FW_BF16: return quant_launch<__nv_bfloat16>(x, M, K, q, s, st);
+    case FW_F16: return quant_launch<__half>(x, M, K, q, s, st);
+    default: return quant_launch<float>(x, M, K, q, s, st);
+  }
+}
+
+int fw_norm_gate_resid(const fw_norm_args* n, void* stream) {
+  using namespace fw;
+  if (!n) return FW_EINVAL;
+  if (n->M < 0 || n->D <= 0 || n->D > FW_NORM_MAX_COLS || n->rows_per_frame <= 0) return FW_ESHAPE;
+  if (n->post < FW_NORM_NONE || n->post > FW_NORM_RMS || n->pre < FW_NORM_NONE || n->pre > FW_NORM_RMS) return FW_EINVAL;
+  if (n->y_dtype != FW_BF16 && n->y_dtype != FW_F32) return FW_EINVAL;
+  if (n->M == 0) return FW_OK;
+  if (!n->resid || (!n->scale) != (!n->shift) || (n->out_s && !n->out) || (!n->y && !n->out)) return FW_EINVAL;
+  if (n->out_s && reinterpret_cast<uintptr_t>(n->out) % 16) return FW_EALIGN;
+  NormArgs a;
+  a.resid = n->resid;
+  a.y = n->y;
+  a.post_w = static_cast<const __nv_bfloat16*>(n->post_w);
+  a.post_b = static_cast<const __nv_bfloat16*>(n->post_b);
+  a.pre_w = static_cast<const __nv_bfloat16*>(n->pre_w);
+  a.pre_b = static_cast<const __nv_bfloat16*>(n->pre_b);
+  a.gate = n->gate;
+  a.shift = n->shift;
+  a.scale = n->scale;
+  a.resid_scale = n->resid_scale;
+  a.branch_scale = n->branch_scale;
+  a.eps = n->eps;
+  a.post = n->post;
+  a.pre = n->pre;
+  a.M = n->M;
+  a.D = n->D;
+  a.rows_per_frame = n->rows_per_frame;
+  a.out = n->out;
+  a.out_s = static_cast<uint8_t*>(n->out_s);
+  // four columns at a time where every row of every tensor starts at a multiple of four elements
+  uintptr_t f32 = 0, b16 = 0;
+  for (const void* p : {(const void*)n->resid, (const void*)n->gate, (const void*)n->shift, (const void*)n->scale,
+                        n->y_dtype == FW_F32 ? n->y : nullptr})
+    f32 |= reinterpret_cast<uintptr_t>(p);
+  for (const void* p : {n->post_w, n->post_b, n->pre_w, n->pre_b, n->y_dtype == FW_BF16 ? n->y : nullptr,
+                        n->out_s ? nullptr : (const void*)n->out})
+    b16 |= reinterpret_cast<uintptr_t>(p);
+  if (f32 % 4 || b16 % 2) return FW_EALIGN;
+  const bool vec = n->D % 4 == 0 && f32 % 16 == 0 && b16 % 8 == 0;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (n->y_dtype == FW_F32) return vec ? norm_launch<float, true>(a, s) : norm_launch<float, false>(a, s);
+  return vec ? norm_launch<__nv_bfloat16, true>(a, s) : norm_launch<__nv_bfloat16, false>(a, s);
+}
+
+}  // extern "C"

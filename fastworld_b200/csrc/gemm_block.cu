@@ -1,0 +1,360 @@
+// Matrix product of block-scaled e4m3 operands (format: fw_block8.cuh) on tcgen05 for sm_100a:
+//   C[m, n] = act(sum over blocks b of 2^(ea[m,b] + eb[n,b]) * sum over k in b of a[m,k] b[n,k] + bias[n])
+// with C in bf16, fp32, or e4m3 with block scales again.
+//
+// The scales are powers of two held as UE8M0 bytes, so tcgen05.mma kind::mxf8f6f4 multiplies them
+// in at full e4m3 rate: its scale factors live in Tensor Memory, one 32-bit word per row (row r of an
+// operand: lane r % 32 of every lane quarter, column r / 32), of which an instruction picks one byte for its 32 of
+// K.  A word here holds the exponents of four blocks of 128, so a word loaded once serves
+// 512 of K: the four instructions of a block name the same byte.
+#include <cmath>
+
+#include "../../include/fastworld_b200.h"
+#include "fw_block8.cuh"
+#include "fw_internal.h"
+
+namespace fw {
+
+namespace {
+
+enum : int { ACT_NONE = 0, ACT_TANH = 1, ACT_ERF = 2 };
+
+struct BlockGemmArgs {
+  int M, N, K;                 // K as padded to 128
+  const uint32_t *sa, *sb;     // exponent words [groups, M], [groups, N]
+  const __nv_bfloat16* bias;   // [N] or null
+  int act, out_dtype;
+  void* out;                   // bf16 / fp32 [M, N], or codes [M, Np]
+  uint8_t* out_s;              // exponents of codes
+};
+
+// Instruction descriptor of kind::mxf8f6f4: e4m3 operands, both K-major, UE8M0 scales (bit 23).
+__host__ __device__ constexpr uint32_t idesc_mx8(int M, int N) {
+  return ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((uint32_t)(M >> 4) << 24);
+}
+// ... with byte `id` of the scale words of both operands
+__device__ __forceinline__ uint32_t with_scale_byte(uint32_t idesc, uint32_t id) { return idesc | (id << 4) | (id << 29); }
+
+__device__ __forceinline__ void umma_mx8(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa,
+                                         uint32_t sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+
+// One 32-bit column per register, this warp's lane quarter.
+template <int N>
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[N]);
+template <>
+__device__ __forceinline__ void tmem_st<1>(uint32_t taddr, const uint32_t (&r)[1]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(r[0]) : "memory");
+}
+template <>
+__device__ __forceinline__ void tmem_st<2>(uint32_t taddr, const uint32_t (&r)[2]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x2.b32 [%0], {%1, %2};" ::"r"(taddr), "r"(r[0]), "r"(r[1]) : "memory");
+}
+template <>
+__device__ __forceinline__ void tmem_st<4>(uint32_t taddr, const uint32_t (&r)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+
+// GELU.  tanh form: 0.5 v (1 + tanh u) = v / (1 + exp(-2u)), within a few fp32 roundings (the
+// hardware's tanh.approx, relative error 2^-11, would show in an fp32 result).  erf form by erfc, which
+// keeps its relative precision where 1 + erf cancels: a block of small negative results is scaled by them.
+__device__ __forceinline__ float act_apply(float v, int act) {
+  if (act == ACT_TANH) {
+    const float u = 0.7978845608028654f * (v + 0.044715f * v * v * v);
+    return v / (1.f + __expf(-2.f * u));
+  }
+  if (act == ACT_ERF) return 0.5f * v * erfcf(v * -0.70710678118654752f);
+  return v;
+}
+
+// ---------------------------------------------------------------- one CTA, 128 columns of C x BN rows
+// The weights' 128 rows are the instruction's M side and BN rows of A its N side, so a few rows
+// cost a small tile (BN = 16) instead of an idle 128-row one, and a tile's 128 columns of C
+// are one block of an e4m3 result.  Warp 0 loads tiles, warp 1 issues the MMAs, warps 2-5
+// carry the exponent words to Tensor Memory, then transpose the accumulator through the
+// (then idle) tile memory and write C a row at a time.
+namespace nk {
+constexpr int THREADS = 192;
+template <int BN>
+struct Cfg {
+  static constexpr int P_BYTES = 128 * 128, Q_BYTES = BN * 128, STAGE = P_BYTES + Q_BYTES;
+  static constexpr int STAGES = BN >= 128 ? 3 : 4;
+  static constexpr int BAR_OFF = STAGES * STAGE;
+  static constexpr int SMEM = BAR_OFF + 256 + 1024;
+  static constexpr int QCOLS = BN >= 32 ? BN / 32 : 1;                // scale columns of the BN rows
+  static constexpr int SF_COL = BN >= 32 ? BN : 32;                   // two buffers of 4 + QCOLS columns, 8 apart
+  static constexpr uint32_t TMEM_COLS = SF_COL + 16 <= 64 ? 64 : SF_COL + 16 <= 128 ? 128 : 256;
+  static_assert(4 + QCOLS <= 8 && SF_COL + 16 <= 256, "scale columns");
+  static_assert(BN * 128 * 4 <= BAR_OFF, "accumulator staging");
+};
+}  // namespace nk
+
+// v: columns [n, n + 4) of row m of C before the bias; columns that do not exist hold anything.
+template <typename F>
+__device__ __forceinline__ void write_row4(const BlockGemmArgs& a, int m, int n, float (&v)[4], F col_bias) {
+  const int N = a.N;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = n + i < N ? act_apply(v[i] + col_bias(i), a.act) : 0.f;
+  if (a.out_dtype == FW_U8) {
+    uint32_t eb;
+    const uint32_t code = b8::encode_block(v, eb);
+    const int Np = b8::padded(N), blk = n / b8::BLK;
+    if (n < Np) *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.out) + (size_t)m * Np + n) = code;
+    if ((threadIdx.x & 31) == 0) {
+      uint8_t* s = a.out_s + ((size_t)(blk / b8::GRP) * a.M + m) * b8::GRP;
+      s[blk % b8::GRP] = (uint8_t)eb;
+      if (blk == b8::blocks(N) - 1)   // places behind the last block
+        for (int j = blk % b8::GRP + 1; j < b8::GRP; ++j) s[j] = 127;
+    }
+    return;
+  }
+  const size_t at = (size_t)m * N + n;
+  if (a.out_dtype == FW_F32) {
+    float* o = static_cast<float*>(a.out) + at;
+    if (N % 4 == 0) {
+      if (n < N) *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n + i < N) o[i] = v[i];
+    }
+  } else {
+    __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.out) + at;
+    if (N % 4 == 0) {
+      if (n < N) *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n + i < N) o[i] = __float2bfloat16_rn(v[i]);
+    }
+  }
+}
+
+template <int BN>
+__global__ void __launch_bounds__(nk::THREADS)
+    gemm_block_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ CUtensorMap tmQ,
+                      const BlockGemmArgs a) {
+  using C = nk::Cfg<BN>;
+  pdl_trigger();
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
+  uint8_t* smem = smem_raw + pad;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
+  uint64_t* empty = full + C::STAGES;
+  uint64_t* sf_full = empty + C::STAGES;   // [2]
+  uint64_t* sf_free = sf_full + 2;         // [2]
+  uint64_t* done = sf_free + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n0 = blockIdx.x * 128, m0 = blockIdx.y * BN;
+  const int kb0 = 0, kb1 = a.K / b8::BLK;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(full + s, 1);
+      mbar_init(empty + s, 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(sf_full + b, 128);
+      mbar_init(sf_free + b, 1);
+    }
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, C::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t used = 0, last_par = 0;
+      for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
+        const int s = i % C::STAGES;
+        const uint32_t par = (uint32_t)(i / C::STAGES) & 1u;
+        if (!mbar_wait(empty + s, par ^ 1u, abort_flag, nullptr, DEV_TIMEOUT_PRODUCER)) break;
+        mbar_arrive_expect_tx(full + s, C::STAGE);
+        tma_load_2d(smem + s * C::STAGE, &tmP, full + s, kb * b8::BLK, n0);
+        tma_load_2d(smem + s * C::STAGE + C::P_BYTES, &tmQ, full + s, kb * b8::BLK, m0);
+        used |= 1u << s;
+        last_par = (last_par & ~(1u << s)) | (par << s);
+      }
+      volatile int no_abort = 0;   // no copy into this CTA's memory is in flight at exit
+      for (int s = 0; s < C::STAGES; ++s)
+        if (used >> s & 1u) mbar_wait(full + s, last_par >> s & 1u, &no_abort, nullptr, DEV_TIMEOUT_DRAIN);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_mx8(128, BN);
+      bool ok = true;
+      for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
+        const int s = i % C::STAGES, grp = kb / b8::GRP - kb0 / b8::GRP, buf = grp & 1;
+        if (i == 0 || kb % b8::GRP == 0)
+          ok = mbar_wait(sf_full + buf, (uint32_t)(grp >> 1) & 1u, abort_flag, nullptr, DEV_TIMEOUT_MMA);
+        if (ok) ok = mbar_wait(full + s, (uint32_t)(i / C::STAGES) & 1u, abort_flag, nullptr, DEV_TIMEOUT_MMA);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t p0 = smem_u32(smem + s * C::STAGE), q0 = p0 + C::P_BYTES;
+        const uint32_t id = with_scale_byte(idesc, (uint32_t)(kb % b8::GRP));
+        const uint32_t sfp = tmem + (uint32_t)(C::SF_COL + buf * 8);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          umma_mx8(tmem, sdesc_sw128(p0 + k * 32, 16, 1024), sdesc_sw128(q0 + k * 32, 16, 1024), id, sfp, sfp + 4,
+                   (i | k) != 0);
+        umma_commit(empty + s);
+        if (kb % b8::GRP == b8::GRP - 1) umma_commit(sf_free + buf);
+      }
+      umma_commit(done);
+      volatile int no_abort = 0;
+      mbar_wait(done, 0, &no_abort, nullptr, DEV_TIMEOUT_DRAIN);
+    }
+  } else {
+    const int q = warp & 3;   // lane quarter of Tensor Memory
+    const uint32_t quarter = tmem + ((uint32_t)(q * 32) << 16);
+    bool ok = true;
+    for (int g = kb0 / b8::GRP, i = 0; g * b8::GRP < kb1; ++g, ++i) {
+      uint32_t wp[4], wq[C::QCOLS];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int r = n0 + c * 32 + lane;
+        wp[c] = r < a.N ? __ldg(a.sb + (size_t)g * a.N + r) : b8::ONES;
+      }
+#pragma unroll
+      for (int c = 0; c < C::QCOLS; ++c) {
+        const int r = m0 + c * 32 + lane;
+        wq[c] = r < a.M && c * 32 + lane < BN ? __ldg(a.sa + (size_t)g * a.M + r) : b8::ONES;
+      }
+      const int buf = i & 1;
+      if (i >= 2) {
+        ok = mbar_wait(sf_free + buf, (uint32_t)((i - 2) >> 1) & 1u, abort_flag, nullptr, DEV_TIMEOUT_PRODUCER);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        tc_fence_after();
+      }
+      tmem_st(quarter + (uint32_t)(C::SF_COL + buf * 8), wp);
+      tmem_st(quarter + (uint32_t)(C::SF_COL + buf * 8 + 4), wq);
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(sf_full + buf);
+    }
+    if (ok) ok = mbar_wait(done, 0, abort_flag, nullptr, DEV_TIMEOUT_EPILOGUE);
+    ok = __all_sync(0xffffffffu, ok);
+    if (ok) {
+      // accumulator lane = column of C, column = row of C; staged as [row][128 columns]
+      tc_fence_after();
+      float* st = reinterpret_cast<float*>(smem);
+      const int col = q * 32 + lane;
+      if constexpr (BN == 16) {
+        uint32_t r[16];
+        tmem_ld16(quarter, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st[i * 128 + col] = __uint_as_float(r[i]);
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < BN / 32; ++c) {
+          uint32_t r[32];
+          tmem_ld32(quarter + (uint32_t)(c * 32), r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) st[(c * 32 + i) * 128 + col] = __uint_as_float(r[i]);
+        }
+      }
+      tc_fence_before();
+    }
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    if (ok) {
+      const float* st = reinterpret_cast<const float*>(smem);
+      const int n = n0 + lane * 4;
+      float bias[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bias[i] = a.bias && n + i < a.N ? __bfloat162float(a.bias[n + i]) : 0.f;
+      for (int r = q; r < BN && m0 + r < a.M; r += 4) {
+        const float4 u = *reinterpret_cast<const float4*>(st + r * 128 + lane * 4);
+        float v[4] = {u.x, u.y, u.z, u.w};
+        write_row4(a, m0 + r, n, v, [&](int i) { return bias[i]; });
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, C::TMEM_COLS);
+  }
+}
+
+template <int BN>
+int launch_nk(const void* A8, const void* B8, const BlockGemmArgs& a, cudaStream_t s) {
+  using C = nk::Cfg<BN>;
+  CUtensorMap tp, tq;
+  int rc = make_tmap_2d(&tp, B8, 1, a.N, a.K, a.K, 128, 128, true);
+  if (!rc) rc = make_tmap_2d(&tq, A8, 1, a.M, a.K, a.K, BN, 128, true);
+  if (rc) return rc;
+  if (cudaFuncSetAttribute(gemm_block_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
+    return FW_ECUDA;
+  const dim3 grid((a.N + 127) / 128, (a.M + BN - 1) / BN);
+  if (grid.y > 65535) return FW_ESHAPE;
+  return launch_k(gemm_block_kernel<BN>, grid, nk::THREADS, C::SMEM, s, tp, tq, a) == cudaSuccess ? FW_OK : FW_ECUDA;
+}
+
+}  // namespace
+}  // namespace fw
+
+extern "C" int fw_gemm_e4m3_block(const void* A8, const void* sa, const void* B8, const void* sb, const void* bias,
+                                  void* out, void* out_s, int M, int N, int K, int epilogue, int out_dtype,
+                                  void* stream) {
+  using namespace fw;
+  if (M < 0 || N < 0 || K <= 0 || K > FW_BLOCK_MAX_COLS || N > FW_BLOCK_MAX_COLS) return FW_ESHAPE;
+  BlockGemmArgs a;
+  switch (epilogue) {
+    case EPI_BF16: a.act = ACT_NONE; break;
+    case EPI_GELU_BF16: a.act = ACT_TANH; break;
+    case EPI_GELU_ERF_BF16: a.act = ACT_ERF; break;
+    default: return FW_EINVAL;
+  }
+  if (out_dtype != FW_BF16 && out_dtype != FW_F32 && out_dtype != FW_U8) return FW_EINVAL;
+  if (M == 0 || N == 0) return FW_OK;
+  if (!A8 || !sa || !B8 || !sb || !out || (out_dtype == FW_U8) != (out_s != nullptr)) return FW_EINVAL;
+  for (const void* p : {A8, B8, (const void*)out})
+    if (reinterpret_cast<uintptr_t>(p) % 16) return FW_EALIGN;
+  for (const void* p : {sa, sb, (const void*)out_s})
+    if (reinterpret_cast<uintptr_t>(p) % 4) return FW_EALIGN;
+  if (reinterpret_cast<uintptr_t>(bias) % 2) return FW_EALIGN;
+  a.M = M;
+  a.N = N;
+  a.K = b8::padded(K);
+  a.sa = static_cast<const uint32_t*>(sa);
+  a.sb = static_cast<const uint32_t*>(sb);
+  a.bias = static_cast<const __nv_bfloat16*>(bias);
+  a.out_dtype = out_dtype;
+  a.out = out;
+  a.out_s = static_cast<uint8_t*>(out_s);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (M <= 16) return launch_nk<16>(A8, B8, a, s);
+  if (M <= 32) return launch_nk<32>(A8, B8, a, s);
+  if (M <= 64) return launch_nk<64>(A8, B8, a, s);
+  return launch_nk<128>(A8, B8, a, s);
+}

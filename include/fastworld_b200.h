@@ -333,6 +333,45 @@ int fw_layernorm(const float* x, int M, int D, float eps, const float* shift, co
  * then _rope at static.py:130-133 in fp32 instead of fp64). */
 int fw_rms_rope(const void* x, int M, int D, float eps, const void* w, const float* rope, int head_dim, void* out,
                 void* stream);
+/* ---- block-scaled e4m3 linears and the norms around them (no counterpart in the reference) ----
+ * The operand format.  x [R, K] is held as codes q [R, Kp] (e4m3 bytes, Kp = K rounded up to 128, zeros
+ * behind K; 16-byte aligned) and exponents s [ceil(Kp / 512), R, 4] (bytes; 4-byte aligned): s[g, r, j] - 127
+ * is the power of two that scales row r's columns [128 (4 g + j), + 128), the smallest one (at least -127)
+ * with max|x| <= 448 * 2^e over the block's finite elements; places behind the last block hold 127.  A
+ * value is code * 2^e; NaN and infinities are held as the NaN code.  At most FW_BLOCK_MAX_COLS columns.
+ * M or N of 0 is a call with nothing to do. */
+#define FW_BLOCK_MAX_COLS (1 << 24)
+/* x [M, K] of `dtype` FW_BF16 / FW_F16 / FW_F32 into q, s. */
+int fw_quant_e4m3_block(const void* x, int dtype, int M, int K, void* q, void* s, void* stream);
+/* out[M, N] = act(A B^T + bias) for A [M, K] (A8, sa) and B [N, K] (B8, sb) in this format, fp32 accumulation;
+ * bias bf16 [N] or NULL.  epilogue: 0 = none, 1 = GELU(tanh), 4 = GELU(erf).  out_dtype: FW_BF16, FW_F32, or
+ * FW_U8 = the same format again (out [M, Np] codes, out_s exponents, quantised from the fp32 result; out_s
+ * is NULL otherwise).  A8, B8 and out 16-byte aligned. */
+int fw_gemm_e4m3_block(const void* A8, const void* sa, const void* B8, const void* sb, const void* bias, void* out,
+                       void* out_s, int M, int N, int K, int epilogue, int out_dtype, void* stream);
+/* The norm after a block, its gate and the residual update, and the norm and modulation before the next:
+ *   b = post(y) * post_w + post_b;   resid = resid_scale * resid + branch_scale * gate[f] * b   (in place)
+ *   out = (pre(resid) * pre_w + pre_b) * (1 + scale[f]) + shift[f]
+ * for fp32 resid [M, D], y [M, D] (FW_BF16 or FW_F32), bf16 weights [D], fp32 gate / scale / shift [frames, D] with
+ * f = row / rows_per_frame; post and pre are FW_NORM_*, fp32 statistics.  Any of the weights and gate may be
+ * NULL (left out), shift and scale both.  y NULL: no residual update; out NULL: no second norm (not both).  out_s
+ * NULL: out is bf16 [M, D]; else out, out_s are the e4m3 format above, quantised from the fp32 result. */
+#define FW_NORM_NONE 0
+#define FW_NORM_LAYER 1
+#define FW_NORM_RMS 2
+#define FW_NORM_MAX_COLS 16384
+typedef struct fw_norm_args {
+  float* resid;
+  const void* y;
+  int y_dtype;
+  int post, pre;
+  const void *post_w, *post_b, *pre_w, *pre_b;
+  const float *gate, *shift, *scale;
+  float resid_scale, branch_scale, eps;
+  int M, D, rows_per_frame;
+  void *out, *out_s;
+} fw_norm_args;
+int fw_norm_gate_resid(const fw_norm_args* args, void* stream);
 /* Non-causal attention, head_dim 128: out[Lq, H*128] = softmax(q k^T / sqrt(128)) v over the
  * keys of segment 0 then segment 1.  meta = device int32 {n_keys0, n_keys1}.  max_keys0/1
  * are the row capacities of the segment buffers. */
