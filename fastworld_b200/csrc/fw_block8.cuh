@@ -41,6 +41,17 @@ __device__ __forceinline__ uint32_t block_exp(uint32_t amax) {
 // 2^-e of a biased exponent byte (at most 247, the byte of the largest fp32 value).
 __device__ __forceinline__ float inv_scale(uint32_t eb) { return __uint_as_float((254u - eb) << 23); }
 
+// Four codes of x * inv where no x is infinite (a NaN becomes the NaN code by itself).
+__device__ __forceinline__ uint32_t encode4_finite(float a, float b, float c, float d, float inv) {
+  const float2 lo2 = __fmul2_rn(make_float2(a, b), make_float2(inv, inv));
+  const float2 hi2 = __fmul2_rn(make_float2(c, d), make_float2(inv, inv));
+  uint32_t r;
+  asm("{\n\t.reg .b16 l, h;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\n\tmov.b32 %0, {l, h};\n\t}"
+      : "=r"(r)
+      : "f"(lo2.x), "f"(lo2.y), "f"(hi2.x), "f"(hi2.y));
+  return r;
+}
 // Four codes of x * inv (round to nearest even; NaN and infinities become the NaN code).
 __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, float inv) {
   auto in = [&](float v) { return (__float_as_uint(v) & 0x7fffffffu) < 0x7f800000u ? v * inv : __uint_as_float(0x7fffffffu); };

@@ -7,79 +7,14 @@
 // operand: lane r % 32 of every lane quarter, column r / 32), of which an instruction picks one byte for its 32 of
 // K.  A word here holds the exponents of four blocks of 128, so a word loaded once serves
 // 512 of K: the four instructions of a block name the same byte.
-#include <cmath>
-
-#include "../../include/fastworld_b200.h"
-#include "fw_block8.cuh"
-#include "fw_internal.h"
+#include "fw_gemm_block.cuh"
 
 namespace fw {
 
 namespace {
 
-enum : int { ACT_NONE = 0, ACT_TANH = 1, ACT_ERF = 2 };
-
-struct BlockGemmArgs {
-  int M, N, K;                 // K as padded to 128
-  const uint32_t *sa, *sb;     // exponent words [groups, M], [groups, N]
-  const __nv_bfloat16* bias;   // [N] or null
-  int act, out_dtype;
-  void* out;                   // bf16 / fp32 [M, N], or codes [M, Np]
-  uint8_t* out_s;              // exponents of codes
-};
-
-// Instruction descriptor of kind::mxf8f6f4: e4m3 operands, both K-major, UE8M0 scales (bit 23).
-__host__ __device__ constexpr uint32_t idesc_mx8(int M, int N) {
-  return ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((uint32_t)(M >> 4) << 24);
-}
-// ... with byte `id` of the scale words of both operands
-__device__ __forceinline__ uint32_t with_scale_byte(uint32_t idesc, uint32_t id) { return idesc | (id << 4) | (id << 29); }
-
-__device__ __forceinline__ void umma_mx8(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa,
-                                         uint32_t sfb, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-      : "memory");
-}
-
-// One 32-bit column per register, this warp's lane quarter.
-template <int N>
-__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[N]);
-template <>
-__device__ __forceinline__ void tmem_st<1>(uint32_t taddr, const uint32_t (&r)[1]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(r[0]) : "memory");
-}
-template <>
-__device__ __forceinline__ void tmem_st<2>(uint32_t taddr, const uint32_t (&r)[2]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x2.b32 [%0], {%1, %2};" ::"r"(taddr), "r"(r[0]), "r"(r[1]) : "memory");
-}
-template <>
-__device__ __forceinline__ void tmem_st<4>(uint32_t taddr, const uint32_t (&r)[4]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
-               "r"(r[2]), "r"(r[3])
-               : "memory");
-}
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-}
-
-// GELU.  tanh form: 0.5 v (1 + tanh u) = v / (1 + exp(-2u)), within a few fp32 roundings (the
-// hardware's tanh.approx, relative error 2^-11, would show in an fp32 result).  erf form by erfc, which
-// keeps its relative precision where 1 + erf cancels: a block of small negative results is scaled by them.
-__device__ __forceinline__ float act_apply(float v, int act) {
-  if (act == ACT_TANH) {
-    const float u = 0.7978845608028654f * (v + 0.044715f * v * v * v);
-    return v / (1.f + __expf(-2.f * u));
-  }
-  if (act == ACT_ERF) return 0.5f * v * erfcf(v * -0.70710678118654752f);
-  return v;
+__device__ __forceinline__ float2 activate(float2 v, int act) {
+  return act == ACT_TANH ? activate2<ACT_TANH>(v) : act == ACT_ERF ? activate2<ACT_ERF>(v) : v;
 }
 
 // ---------------------------------------------------------------- one CTA, 128 columns of C x BN rows
@@ -109,7 +44,11 @@ template <typename F>
 __device__ __forceinline__ void write_row4(const BlockGemmArgs& a, int m, int n, float (&v)[4], F col_bias) {
   const int N = a.N;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = n + i < N ? act_apply(v[i] + col_bias(i), a.act) : 0.f;
+  for (int i = 0; i < 4; i += 2) {
+    const float2 u = activate(make_float2(v[i] + col_bias(i), v[i + 1] + col_bias(i + 1)), a.act);
+    v[i] = n + i < N ? u.x : 0.f;
+    v[i + 1] = n + i + 1 < N ? u.y : 0.f;
+  }
   if (a.out_dtype == FW_U8) {
     uint32_t eb;
     const uint32_t code = b8::encode_block(v, eb);
@@ -194,7 +133,7 @@ __global__ void __launch_bounds__(nk::THREADS)
       for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
         const int s = i % C::STAGES;
         const uint32_t par = (uint32_t)(i / C::STAGES) & 1u;
-        if (!mbar_wait(empty + s, par ^ 1u, abort_flag, nullptr, DEV_TIMEOUT_PRODUCER)) break;
+        if (!wait_on(empty + s, par ^ 1u, abort_flag)) break;
         mbar_arrive_expect_tx(full + s, C::STAGE);
         tma_load_2d(smem + s * C::STAGE, &tmP, full + s, kb * b8::BLK, n0);
         tma_load_2d(smem + s * C::STAGE + C::P_BYTES, &tmQ, full + s, kb * b8::BLK, m0);
@@ -206,27 +145,25 @@ __global__ void __launch_bounds__(nk::THREADS)
         if (used >> s & 1u) mbar_wait(full + s, last_par >> s & 1u, &no_abort, nullptr, DEV_TIMEOUT_DRAIN);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    {
+      const uint32_t one = lane == 0;
       constexpr uint32_t idesc = idesc_mx8(128, BN);
       bool ok = true;
       for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
         const int s = i % C::STAGES, grp = kb / b8::GRP - kb0 / b8::GRP, buf = grp & 1;
         if (i == 0 || kb % b8::GRP == 0)
-          ok = mbar_wait(sf_full + buf, (uint32_t)(grp >> 1) & 1u, abort_flag, nullptr, DEV_TIMEOUT_MMA);
-        if (ok) ok = mbar_wait(full + s, (uint32_t)(i / C::STAGES) & 1u, abort_flag, nullptr, DEV_TIMEOUT_MMA);
+          ok = wait_on(sf_full + buf, (uint32_t)(grp >> 1) & 1u, abort_flag);
+        if (ok) ok = wait_on(full + s, (uint32_t)(i / C::STAGES) & 1u, abort_flag);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t p0 = smem_u32(smem + s * C::STAGE), q0 = p0 + C::P_BYTES;
-        const uint32_t id = with_scale_byte(idesc, (uint32_t)(kb % b8::GRP));
-        const uint32_t sfp = tmem + (uint32_t)(C::SF_COL + buf * 8);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          umma_mx8(tmem, sdesc_sw128(p0 + k * 32, 16, 1024), sdesc_sw128(q0 + k * 32, 16, 1024), id, sfp, sfp + 4,
-                   (i | k) != 0);
-        umma_commit(empty + s);
-        if (kb % b8::GRP == b8::GRP - 1) umma_commit(sf_free + buf);
+        const uint32_t desc = desc_lo(smem_u32(smem + s * C::STAGE));
+        const uint32_t sf = tmem + (uint32_t)(C::SF_COL + buf * 8);
+        umma_mx8_block<1>(one, tmem, desc, desc + (C::P_BYTES >> 4), with_scale_byte(idesc, (uint32_t)(kb % b8::GRP)), sf, sf + 4,
+                          i != 0);
+        umma_commit_if<1>(one, empty + s);
+        if (kb % b8::GRP == b8::GRP - 1) umma_commit_if<1>(one, sf_free + buf);
       }
-      umma_commit(done);
+      umma_commit_if<1>(one, done);
       volatile int no_abort = 0;
       mbar_wait(done, 0, &no_abort, nullptr, DEV_TIMEOUT_DRAIN);
     }
@@ -248,8 +185,8 @@ __global__ void __launch_bounds__(nk::THREADS)
       }
       const int buf = i & 1;
       if (i >= 2) {
-        ok = mbar_wait(sf_free + buf, (uint32_t)((i - 2) >> 1) & 1u, abort_flag, nullptr, DEV_TIMEOUT_PRODUCER);
-        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        ok = __all_sync(0xffffffffu, wait_on(sf_free + buf, (uint32_t)((i - 2) >> 1) & 1u, abort_flag));
+        if (!ok) break;
         tc_fence_after();
       }
       tmem_st(quarter + (uint32_t)(C::SF_COL + buf * 8), wp);
@@ -258,8 +195,7 @@ __global__ void __launch_bounds__(nk::THREADS)
       tc_fence_before();
       mbar_arrive(sf_full + buf);
     }
-    if (ok) ok = mbar_wait(done, 0, abort_flag, nullptr, DEV_TIMEOUT_EPILOGUE);
-    ok = __all_sync(0xffffffffu, ok);
+    if (ok) ok = __all_sync(0xffffffffu, wait_on(done, 0, abort_flag));
     if (ok) {
       // accumulator lane = column of C, column = row of C; staged as [row][128 columns]
       tc_fence_after();
@@ -353,6 +289,7 @@ extern "C" int fw_gemm_e4m3_block(const void* A8, const void* sa, const void* B8
   a.out = out;
   a.out_s = static_cast<uint8_t*>(out_s);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (M > 512) return gemm_block_wide_launch(A8, B8, a, s);
   if (M <= 16) return launch_nk<16>(A8, B8, a, s);
   if (M <= 32) return launch_nk<32>(A8, B8, a, s);
   if (M <= 64) return launch_nk<64>(A8, B8, a, s);

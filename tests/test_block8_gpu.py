@@ -50,6 +50,12 @@ def value(q, s):
     return (q.view(F8).double().view(r, -1, 128) * pow2(e)[..., None]).view(r, kp)
 
 
+def powers(lo, hi, *shape, seed=0):
+    """Random powers of two, exponents in [lo, hi)."""
+    g = torch.Generator(device="cuda").manual_seed(seed + 91)
+    return torch.exp2(torch.randint(lo, hi, shape, device="cuda", generator=g).float())
+
+
 def rand(*shape, seed=0, dtype=torch.bfloat16, size=1.0):
     g = torch.Generator(device="cuda").manual_seed(seed + sum(shape) * 7)
     return (torch.randn(*shape, device="cuda", generator=g) * size).to(dtype)
@@ -65,7 +71,7 @@ def is_nan_code(q):
                                  (1001, 640)])
 def test_quant_exact(M, K, dtype):
     from fastworld_b200 import ops
-    x = rand(M, K, dtype=dtype) * torch.exp2(torch.randint(-12, 12, (M, 1), device="cuda")).to(dtype)
+    x = rand(M, K, dtype=dtype) * powers(-12, 12, M, 1).to(dtype)
     q, s = ops.quant_e4m3_block(x)
     rq, rs = ref_quant(x)
     assert torch.equal(s, rs)
@@ -106,16 +112,17 @@ def test_quant_unaligned_view_and_empty():
 # ---------------------------------------------------------------- product
 def act64(v, name):
     if name == "gelu_tanh":
-        return 0.5 * v * (1 + torch.tanh(math.sqrt(2 / math.pi) * (v + 0.044715 * v ** 3)))
+        # 0.5 (1 + tanh u) = sigmoid(2u): the sum cancels below u = -18 even in fp64
+        return v * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (v + 0.044715 * v ** 3))
     return 0.5 * v * torch.special.erfc(-v * math.sqrt(0.5)) if name == "gelu_erf" else v
 
 
 def operands(M, N, K, seed=0):
     from fastworld_b200 import ops
-    a = rand(M, K, seed=seed, size=1.0) * torch.exp2(torch.randint(-3, 4, (M, 1), device="cuda")).bfloat16()
+    a = rand(M, K, seed=seed, size=1.0) * powers(-3, 4, M, 1, seed=seed).bfloat16()
     b = rand(N, K, seed=seed + 1, size=1 / math.sqrt(K))
     # blocks of very different size, so that a wrong scale shows
-    blk = torch.exp2(torch.randint(-4, 5, (-(-K // 128),), device="cuda").float()).repeat_interleave(128)[:K]
+    blk = powers(-4, 5, -(-K // 128), seed=seed + 1).repeat_interleave(128)[:K]
     a, b = (a * blk).bfloat16(), (b * blk.flip(0)).bfloat16()
     return (*ops.quant_e4m3_block(a), *ops.quant_e4m3_block(b))
 
@@ -188,6 +195,24 @@ def test_gemm_scales_at_the_ends():
     assert got[3].isnan().all()
     keep = torch.arange(M, device="cuda") != 3
     assert torch.equal(got[keep], base[keep])
+
+
+@pytest.mark.parametrize("M,N,K", [(20, 300, 256), (600, 300, 256), (1500, 1000, 640)])
+@pytest.mark.parametrize("out", ["f32", "e4m3"])
+def test_gemm_infinities(M, N, K, out):
+    """A result that overflows fp32 is an infinity, the NaN code in e4m3; its block is scaled by what is finite."""
+    from fastworld_b200 import ops
+    a8, sa, b8, sb = operands(M, N, K, seed=5)
+    sa[:, 7] = 127 + 70
+    sb[:, N - 3:] = 127 + 70                           # (7, N - 3 ...): 2^140 times a sum; 2^70 elsewhere
+    v = ops.gemm_e4m3_block(a8, sa, b8, sb, out="f32")
+    assert v[7, N - 3:].isinf().all() and v[:7].isfinite().all() and v[8:].isfinite().all()
+    if out == "e4m3":
+        q, s = ops.gemm_e4m3_block(a8, sa, b8, sb, out="e4m3")
+        rq, rs = ref_quant(v)
+        assert torch.equal(s, rs) and torch.equal(is_nan_code(q), is_nan_code(rq))
+        keep = ~is_nan_code(rq)
+        assert torch.equal(q[keep], rq[keep])
 
 
 def test_gemm_no_rows():
