@@ -13,6 +13,7 @@ struct BlockGemmArgs {
   const uint32_t *sa, *sb;     // exponent words [groups, M], [groups, N]
   const __nv_bfloat16* bias;   // [N] or null
   int act, out_dtype;
+  int splits;                  // CTAs that share a tile's k-blocks (gemm_block.cu)
   void* out;                   // bf16 / fp32 [M, N], or codes [M, Np]
   uint8_t* out_s;              // exponents of codes
 };

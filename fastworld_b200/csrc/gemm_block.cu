@@ -9,6 +9,8 @@
 // 512 of K: the four instructions of a block name the same byte.
 #include "fw_gemm_block.cuh"
 
+#include <cmath>
+
 namespace fw {
 
 namespace {
@@ -22,9 +24,13 @@ __device__ __forceinline__ float2 activate(float2 v, int act) {
 // cost a small tile (BN = 16) instead of an idle 128-row one, and a tile's 128 columns of C
 // are one block of an e4m3 result.  Warp 0 loads tiles, warp 1 issues the MMAs, warps 2-5
 // carry the exponent words to Tensor Memory, then transpose the accumulator through the
-// (then idle) tile memory and write C a row at a time.
+// (then idle) tile memory; all warps write C a row at a time.
+//
+// Few tiles would leave most SMs idle and stream the weights through few of them, so the k-blocks of a tile are
+// split over a cluster of CTAs.  Each stages its partial accumulator in its own shared memory; then each takes
+// every splits-th row, adds the partials of all ranks in rank order (the same sum on every run) and writes it.
 namespace nk {
-constexpr int THREADS = 192;
+constexpr int THREADS = 192, MAX_SPLITS = 8;
 template <int BN>
 struct Cfg {
   static constexpr int P_BYTES = 128 * 128, Q_BYTES = BN * 128, STAGE = P_BYTES + Q_BYTES;
@@ -39,13 +45,18 @@ struct Cfg {
 };
 }  // namespace nk
 
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {   // shared memory of a CTA of the cluster
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
 // v: columns [n, n + 4) of row m of C before the bias; columns that do not exist hold anything.
-template <typename F>
-__device__ __forceinline__ void write_row4(const BlockGemmArgs& a, int m, int n, float (&v)[4], F col_bias) {
+__device__ __forceinline__ void write_row4(const BlockGemmArgs& a, int m, int n, float (&v)[4], const float (&bias)[4]) {
   const int N = a.N;
 #pragma unroll
   for (int i = 0; i < 4; i += 2) {
-    const float2 u = activate(make_float2(v[i] + col_bias(i), v[i + 1] + col_bias(i + 1)), a.act);
+    const float2 u = activate(make_float2(v[i] + bias[i], v[i + 1] + bias[i + 1]), a.act);
     v[i] = n + i < N ? u.x : 0.f;
     v[i + 1] = n + i + 1 < N ? u.y : 0.f;
   }
@@ -101,8 +112,9 @@ __global__ void __launch_bounds__(nk::THREADS)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n0 = blockIdx.x * 128, m0 = blockIdx.y * BN;
-  const int kb0 = 0, kb1 = a.K / b8::BLK;
+  const int splits = a.splits, rank = splits > 1 ? (int)cluster_ctarank() : 0;
+  const int n0 = (int)(blockIdx.x / splits) * 128, m0 = blockIdx.y * BN;
+  const int num_kb = a.K / b8::BLK, kb0 = num_kb * rank / splits, kb1 = num_kb * (rank + 1) / splits;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
@@ -219,22 +231,36 @@ __global__ void __launch_bounds__(nk::THREADS)
       }
       tc_fence_before();
     }
-    asm volatile("bar.sync 1, 128;" ::: "memory");
-    if (ok) {
-      const float* st = reinterpret_cast<const float*>(smem);
-      const int n = n0 + lane * 4;
-      float bias[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) bias[i] = a.bias && n + i < a.N ? __bfloat162float(a.bias[n + i]) : 0.f;
-      for (int r = q; r < BN && m0 + r < a.M; r += 4) {
-        const float4 u = *reinterpret_cast<const float4*>(st + r * 128 + lane * 4);
-        float v[4] = {u.x, u.y, u.z, u.w};
-        write_row4(a, m0 + r, n, v, [&](int i) { return bias[i]; });
-      }
-    }
+    if (!ok) *abort_flag = 1;
   }
   tc_fence_before();
-  __syncthreads();
+  __syncthreads();   // the partial accumulator is staged
+  if (splits > 1) cluster_sync();
+  if (!*abort_flag) {
+    const int n = n0 + lane * 4;
+    float bias[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bias[i] = a.bias && n + i < a.N ? __bfloat162float(a.bias[n + i]) : 0.f;
+    for (int r = warp * splits + rank; r < BN && m0 + r < a.M; r += nk::THREADS / 32 * splits) {
+      const float* at = reinterpret_cast<const float*>(smem) + r * 128 + lane * 4;
+      float v[4];
+      if (splits == 1) {
+        const float4 u = *reinterpret_cast<const float4*>(at);
+        v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
+      } else {
+        float4 u[nk::MAX_SPLITS];
+#pragma unroll
+        for (int k = 0; k < nk::MAX_SPLITS; ++k)
+          if (k < splits) u[k] = ld_cluster4(mapa_cluster(at, (uint32_t)k));
+        v[0] = u[0].x, v[1] = u[0].y, v[2] = u[0].z, v[3] = u[0].w;
+#pragma unroll
+        for (int k = 1; k < nk::MAX_SPLITS; ++k)
+          if (k < splits) v[0] += u[k].x, v[1] += u[k].y, v[2] += u[k].z, v[3] += u[k].w;
+      }
+      write_row4(a, m0 + r, n, v, bias);
+    }
+  }
+  if (splits > 1) cluster_sync();   // no CTA leaves while another reads its partial
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
@@ -251,9 +277,66 @@ int launch_nk(const void* A8, const void* B8, const BlockGemmArgs& a, cudaStream
   if (rc) return rc;
   if (cudaFuncSetAttribute(gemm_block_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
     return FW_ECUDA;
-  const dim3 grid((a.N + 127) / 128, (a.M + BN - 1) / BN);
+  const dim3 grid((a.N + 127) / 128 * a.splits, (a.M + BN - 1) / BN);
   if (grid.y > 65535) return FW_ESHAPE;
-  return launch_k(gemm_block_kernel<BN>, grid, nk::THREADS, C::SMEM, s, tp, tq, a) == cudaSuccess ? FW_OK : FW_ECUDA;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = nk::THREADS;
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  cfg.attrs = attr;
+  if (a.splits > 1) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = a.splits;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.numAttrs = 1;
+  }
+  if (pdl_enabled()) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_block_kernel<BN>, tp, tq, a);
+  note_launch();
+  return e == cudaSuccess ? FW_OK : FW_ECUDA;
+}
+
+// Which kernel, tile and split: the least of a time model (us) whose constants were fitted to 70 measured
+// sizes (1 to 4000 rows, 30 to 13824 columns, 60 to 8960 of K): its choice is 3 % off the best variant on
+// average.  Small tiles: launch, then the busiest SM's operand bytes, or the latency of a CTA's chain of
+// k-blocks, or HBM, then the exposed epilogue and the join of a split; wide kernel: waves of 256 x 256 tiles.
+// Both sides, measured: 880 x 1536 x 8960 18.4 us on 128-row tiles split 3 ways, 31.2 us wide; 2640 x 1536 x 1536
+// 14.1 and 11.0 us; 512 x 1536 x 4096 11.8 us split 5 ways, 19.3 us unsplit, 17.9 us wide; 1 x 9216 x 1536 6.8 us
+// split 4 ways, 7.3 us unsplit.  A split's CTAs are at most two per SM: more would wait for whole tiles to end.
+struct Plan {
+  int bn, splits;   // bn 0: the wide kernel
+};
+Plan make_plan(int M, int N, int num_kb, int out_dtype) {
+  const int sms = num_sms();
+  auto up = [](long long x, long long y) { return (x + y - 1) / y; };
+  const double hbm = (((double)M + N) * num_kb * b8::BLK + 2.0 * M * N) / 5.2e6;
+  const long long waves = up(up(M, 256) * up(N, 256), sms / 2);
+  const bool tma_out = out_dtype == FW_U8 || N % (out_dtype == FW_F32 ? 4 : 8) == 0;
+  Plan best = {0, 1};
+  double least = 4.0 + waves * (num_kb * 0.6 + (tma_out ? 1.0 : 3.5)) - 1.0;
+  for (int bn = 16; bn <= 128; bn *= 2) {
+    if (up(M, bn) > 65535) continue;
+    const long long tiles = up(N, 128) * up(M, bn);
+    for (int sp = 1; sp <= nk::MAX_SPLITS && sp <= num_kb; ++sp) {
+      if (sp > 1 && tiles * sp > 2 * sms) break;
+      const double per_sm = (double)up(tiles * sp, sms), kbs = (double)up(num_kb, sp);
+      const double load = per_sm * kbs * (128 + bn) * b8::BLK / 6.0e4;
+      const double chain = up(tiles * sp, 2 * sms) * kbs * 0.18;
+      const double t = 3.0 + fmax(fmax(load, chain), hbm) + 1.1 * bn / 128 * per_sm + (sp > 1 ? 0.9 : 0.0);
+      if (t < least) {
+        least = t;
+        best = {bn, sp};
+      }
+    }
+    if (bn >= M) break;   // one tile of rows
+  }
+  return best;
 }
 
 }  // namespace
@@ -289,9 +372,13 @@ extern "C" int fw_gemm_e4m3_block(const void* A8, const void* sa, const void* B8
   a.out = out;
   a.out_s = static_cast<uint8_t*>(out_s);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (M > 512) return gemm_block_wide_launch(A8, B8, a, s);
-  if (M <= 16) return launch_nk<16>(A8, B8, a, s);
-  if (M <= 32) return launch_nk<32>(A8, B8, a, s);
-  if (M <= 64) return launch_nk<64>(A8, B8, a, s);
-  return launch_nk<128>(A8, B8, a, s);
+  const Plan p = make_plan(M, N, a.K / b8::BLK, out_dtype);
+  a.splits = p.splits;
+  switch (p.bn) {
+    case 16: return launch_nk<16>(A8, B8, a, s);
+    case 32: return launch_nk<32>(A8, B8, a, s);
+    case 64: return launch_nk<64>(A8, B8, a, s);
+    case 128: return launch_nk<128>(A8, B8, a, s);
+    default: return gemm_block_wide_launch(A8, B8, a, s);
+  }
 }

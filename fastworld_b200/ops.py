@@ -139,24 +139,15 @@ def rms_rope(x: torch.Tensor, w: torch.Tensor, rope=None, head_dim: int = 128, e
 # An operand x [R, K] is a pair (q, s): e4m3 codes q [R, Kp] (uint8; Kp = K rounded up to 128, zeros behind
 # K) and exponents s [ceil(Kp / 512), R, 4] (uint8): s[g, r, j] - 127 is the power of two that scales
 # row r's columns [128 (4 g + j), + 128); places behind the last block hold 127.
-def _on(dev, fn, what, *args):
-    """fn(*args, stream) on dev's current stream, with dev as the current device."""
-    if torch.cuda.current_device() == dev.index:
-        check(fn(*args, stream_ptr()), what)
+def _on(index, fn, what, *args):
+    """fn(*args, stream) on the current stream of device `index`, with that device as the current one."""
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(dev):
-            check(fn(*args, stream_ptr()), what)
-
-
-def _same_device(dev, **tensors):
-    for n, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise ValueError(f"{n}: on {t.device}, expected {dev}")
-
-
-def _shape(t, shape, name):
-    if tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc, what)
 
 
 def _block_empty(rows, cols, dev):
@@ -166,28 +157,26 @@ def _block_empty(rows, cols, dev):
             torch.empty(-(-kp // 512), rows, 4, device=dev, dtype=torch.uint8))
 
 
-def _block_req(q, s, name):
-    """Checks an operand's codes and exponents; returns its rows and padded columns."""
-    _req(q, torch.uint8, name + "8")
-    _req(s, torch.uint8, "s" + name)
-    if q.ndim != 2 or q.shape[1] == 0 or q.shape[1] % 128:
-        raise ValueError(f"{name}8: shape {tuple(q.shape)}, expected [rows, a positive multiple of 128]")
-    _shape(s, (-(-q.shape[1] // 512), q.shape[0], 4), "s" + name)
-    return q.shape
+def _is(t, dtype, index):
+    return t.dtype is dtype and t.get_device() == index and t.is_contiguous()
+
+
+def _refuse(name, t, dtype, index, shape):
+    where = f"cuda:{index}" if index >= 0 else "a CUDA device"
+    raise ValueError(f"{name}: expected a contiguous {dtype} tensor of shape {shape} on {where}, got {t.dtype} "
+                     f"{tuple(t.shape)} with strides {t.stride()} on {t.device}")
 
 
 def quant_e4m3_block(x: torch.Tensor):
     """x [M, K] (bf16, fp16 or fp32) in block-scaled e4m3: (q [M, Kp], s [ceil(Kp / 512), M, 4]), both
     uint8.  Each row's 128 columns share the smallest power of two 2^e (e >= -127) with
     max|x| <= 448 * 2^e over the finite elements; NaN and infinities become the NaN code."""
-    if x.dtype not in _DTYPES:
-        raise ValueError(f"x: expected bf16, fp16 or fp32, got {x.dtype}")
-    _req(x, x.dtype, "x")
-    if x.ndim != 2 or x.shape[1] == 0:
-        raise ValueError(f"x: shape {tuple(x.shape)}, expected [M, K] with K > 0")
-    M, K = x.shape
+    dtype, index, shape = _DTYPES.get(x.dtype), x.get_device(), x.shape
+    if dtype is None or index < 0 or len(shape) != 2 or shape[1] == 0 or not x.is_contiguous():
+        _refuse("x", x, "bf16, fp16 or fp32", index, "[M, K > 0]")
+    M, K = shape
     q, s = _block_empty(M, K, x.device)
-    _on(x.device, lib().fw_quant_e4m3_block, "quant_e4m3_block", ptr(x), _DTYPES[x.dtype], M, K, ptr(q), ptr(s))
+    _on(index, lib().fw_quant_e4m3_block, "quant_e4m3_block", x.data_ptr(), dtype, M, K, q.data_ptr(), s.data_ptr())
     return q, s
 
 
@@ -200,14 +189,20 @@ def gemm_e4m3_block(a8: torch.Tensor, sa: torch.Tensor, b8: torch.Tensor, sb: to
         raise ValueError(f"epilogue: {epilogue!r}, expected one of {sorted(BLOCK_EPILOGUES)}")
     if out not in BLOCK_OUTPUTS:
         raise ValueError(f"out: {out!r}, expected one of {sorted(BLOCK_OUTPUTS)}")
-    M, K = _block_req(a8, sa, "a")
-    N, Kb = _block_req(b8, sb, "b")
-    if K != Kb:
-        raise ValueError(f"a8 and b8 have {K} and {Kb} columns")
-    if bias is not None:
-        _req(bias, torch.bfloat16, "bias")
-        _shape(bias, (N,), "bias")
-    _same_device(a8.device, sa=sa, b8=b8, sb=sb, bias=bias)
+    u8, index, shape = torch.uint8, a8.get_device(), a8.shape
+    if index < 0 or len(shape) != 2 or shape[1] == 0 or shape[1] % 128 or not _is(a8, u8, index):
+        _refuse("a8", a8, u8, index, "[M, a positive multiple of 128]")
+    M, K = shape
+    shape = b8.shape
+    if len(shape) != 2 or shape[1] != K or not _is(b8, u8, index):
+        _refuse("b8", b8, u8, index, f"[N, {K}]")
+    N, groups = shape[0], -(-K // 512)
+    if sa.shape != (groups, M, 4) or not _is(sa, u8, index):
+        _refuse("sa", sa, u8, index, [groups, M, 4])
+    if sb.shape != (groups, N, 4) or not _is(sb, u8, index):
+        _refuse("sb", sb, u8, index, [groups, N, 4])
+    if bias is not None and (bias.shape != (N,) or not _is(bias, torch.bfloat16, index)):
+        _refuse("bias", bias, torch.bfloat16, index, [N])
     code, dtype = BLOCK_OUTPUTS[out]
     if out == "e4m3":
         if N == 0:
@@ -215,8 +210,8 @@ def gemm_e4m3_block(a8: torch.Tensor, sa: torch.Tensor, b8: torch.Tensor, sb: to
         o, so = _block_empty(M, N, a8.device)
     else:
         o, so = torch.empty(M, N, device=a8.device, dtype=dtype), None
-    _on(a8.device, lib().fw_gemm_e4m3_block, "gemm_e4m3_block", ptr(a8), ptr(sa), ptr(b8), ptr(sb), ptr(bias), ptr(o),
-        ptr(so), M, N, K, BLOCK_EPILOGUES[epilogue], code)
+    _on(index, lib().fw_gemm_e4m3_block, "gemm_e4m3_block", a8.data_ptr(), sa.data_ptr(), b8.data_ptr(), sb.data_ptr(),
+        ptr(bias), o.data_ptr(), ptr(so), M, N, K, BLOCK_EPILOGUES[epilogue], code)
     return o if so is None else (o, so)
 
 
@@ -232,10 +227,10 @@ def norm_gate_resid_(resid: torch.Tensor, y=None, post=None, post_w=None, post_b
     fp32 statistics; weights bf16 [D]; gate, shift and scale fp32 [frames, D] (or [D], one frame) with
     f = row // rows_per_frame (None: all rows are one frame).  out: 'bf16', 'e4m3' (the pair (q, s) of
     quant_e4m3_block, quantised from fp32) or None (h is not computed)."""
-    _req(resid, torch.float32, "resid")
-    if resid.ndim != 2 or resid.shape[1] == 0:
-        raise ValueError(f"resid: shape {tuple(resid.shape)}, expected [M, D] with D > 0")
-    M, D = resid.shape
+    f32, b16, index, shape = torch.float32, torch.bfloat16, resid.get_device(), resid.shape
+    if index < 0 or len(shape) != 2 or shape[1] == 0 or not _is(resid, f32, index):
+        _refuse("resid", resid, f32, index, "[M, D > 0]")
+    M, D = shape
     if post not in NORMS or pre not in NORMS:
         raise ValueError(f"post, pre: {post!r}, {pre!r}, expected 'layer', 'rms' or None")
     if out not in ("bf16", "e4m3", None):
@@ -252,31 +247,24 @@ def norm_gate_resid_(resid: torch.Tensor, y=None, post=None, post_w=None, post_b
     rpf = max(M, 1) if rows_per_frame is None else int(rows_per_frame)
     if rpf <= 0:
         raise ValueError(f"rows_per_frame: {rows_per_frame}")
-    if y is not None:
-        if y.dtype not in (torch.bfloat16, torch.float32):
-            raise ValueError(f"y: expected bf16 or fp32, got {y.dtype}")
-        _req(y, y.dtype, "y")
-        _shape(y, (M, D), "y")
+    if y is not None and (y.dtype not in (b16, f32) or y.shape != shape or not _is(y, y.dtype, index)):
+        _refuse("y", y, "bf16 or fp32", index, [M, D])
     for n, t in (("post_w", post_w), ("post_b", post_b), ("pre_w", pre_w), ("pre_b", pre_b)):
-        if t is not None:
-            _req(t, torch.bfloat16, n)
-            _shape(t, (D,), n)
+        if t is not None and (t.shape != (D,) or not _is(t, b16, index)):
+            _refuse(n, t, b16, index, [D])
     frames = -(-M // rpf)
     for n, t in (("gate", gate), ("shift", shift), ("scale", scale)):
         if t is not None:
-            _req(t, torch.float32, n)
-            rows = 1 if t.ndim == 1 else t.shape[0]
-            if t.ndim not in (1, 2) or t.shape[-1] != D or rows < frames:
-                raise ValueError(f"{n}: shape {tuple(t.shape)}, expected [{frames}, {D}]" + (f" or [{D}]" * (frames <= 1)))
-    _same_device(resid.device, y=y, post_w=post_w, post_b=post_b, gate=gate, pre_w=pre_w, pre_b=pre_b, shift=shift,
-                 scale=scale)
+            ts = t.shape
+            if not (len(ts) == 2 and ts[0] >= frames or len(ts) == 1 and frames <= 1) or ts[-1] != D or not _is(t, f32, index):
+                _refuse(n, t, f32, index, f"[{frames}, {D}]" + (f" or [{D}]" if frames <= 1 else ""))
     h = s = None
     if out == "e4m3":
         h, s = _block_empty(M, D, resid.device)
     elif out == "bf16":
         h = torch.empty(M, D, device=resid.device, dtype=torch.bfloat16)
-    a = _lib.FwNormArgs(ptr(resid), ptr(y), _DTYPES[torch.bfloat16 if y is None else y.dtype], NORMS[post], NORMS[pre],
+    a = _lib.FwNormArgs(resid.data_ptr(), ptr(y), _lib.DT_BF16 if y is None else _DTYPES[y.dtype], NORMS[post], NORMS[pre],
                         ptr(post_w), ptr(post_b), ptr(pre_w), ptr(pre_b), ptr(gate), ptr(shift), ptr(scale),
                         resid_scale, branch_scale, eps, M, D, min(rpf, 2**31 - 1), ptr(h), ptr(s))
-    _on(resid.device, lib().fw_norm_gate_resid, "norm_gate_resid", ctypes.byref(a))
+    _on(index, lib().fw_norm_gate_resid, "norm_gate_resid", ctypes.byref(a))
     return (h, s) if out == "e4m3" else h
