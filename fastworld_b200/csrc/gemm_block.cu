@@ -10,14 +10,11 @@
 #include "fw_gemm_block.cuh"
 
 #include <cmath>
+#include <type_traits>
 
 namespace fw {
 
 namespace {
-
-__device__ __forceinline__ float2 activate(float2 v, int act) {
-  return act == ACT_TANH ? activate2<ACT_TANH>(v) : act == ACT_ERF ? activate2<ACT_ERF>(v) : v;
-}
 
 // ---------------------------------------------------------------- one CTA, 128 columns of C x BN rows
 // The weights' 128 rows are the instruction's M side and BN rows of A its N side, so a few rows
@@ -47,55 +44,59 @@ struct Cfg {
 
 __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {   // shared memory of a CTA of the cluster
   float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
   return v;
 }
 
 // v: columns [n, n + 4) of row m of C before the bias; columns that do not exist hold anything.
-__device__ __forceinline__ void write_row4(const BlockGemmArgs& a, int m, int n, float (&v)[4], const float (&bias)[4]) {
+template <int ACT, int OUT>
+__device__ __forceinline__ void write_row4(const BlockGemmArgs& a, int m, int n, const float4& u, const float (&bias)[4],
+                                           bool vec) {
   const int N = a.N;
-#pragma unroll
-  for (int i = 0; i < 4; i += 2) {
-    const float2 u = activate(make_float2(v[i] + bias[i], v[i + 1] + bias[i + 1]), a.act);
-    v[i] = n + i < N ? u.x : 0.f;
-    v[i + 1] = n + i + 1 < N ? u.y : 0.f;
-  }
-  if (a.out_dtype == FW_U8) {
+  const float2 x = activate2<ACT>(make_float2(u.x + bias[0], u.y + bias[1]));
+  const float2 y = activate2<ACT>(make_float2(u.z + bias[2], u.w + bias[3]));
+  if constexpr (OUT == FW_U8) {
+    const float v[4] = {n < N ? x.x : 0.f, n + 1 < N ? x.y : 0.f, n + 2 < N ? y.x : 0.f, n + 3 < N ? y.y : 0.f};
     uint32_t eb;
     const uint32_t code = b8::encode_block(v, eb);
-    const int Np = b8::padded(N), blk = n / b8::BLK;
-    if (n < Np) *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.out) + (size_t)m * Np + n) = code;
+    const int blk = n / b8::BLK;
+    *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.out) + (size_t)m * b8::padded(N) + n) = code;
     if ((threadIdx.x & 31) == 0) {
       uint8_t* s = a.out_s + ((size_t)(blk / b8::GRP) * a.M + m) * b8::GRP;
       s[blk % b8::GRP] = (uint8_t)eb;
       if (blk == b8::blocks(N) - 1)   // places behind the last block
         for (int j = blk % b8::GRP + 1; j < b8::GRP; ++j) s[j] = 127;
     }
-    return;
-  }
-  const size_t at = (size_t)m * N + n;
-  if (a.out_dtype == FW_F32) {
-    float* o = static_cast<float*>(a.out) + at;
-    if (N % 4 == 0) {
-      if (n < N) *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (n + i < N) o[i] = v[i];
-    }
   } else {
-    __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.out) + at;
-    if (N % 4 == 0) {
-      if (n < N) *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+    const size_t at = (size_t)m * N + n;
+    if constexpr (OUT == FW_F32) {
+      float* o = static_cast<float*>(a.out) + at;
+      if (vec) {
+        *reinterpret_cast<float4*>(o) = make_float4(x.x, x.y, y.x, y.y);
+      } else {
+        if (n < N) o[0] = x.x;
+        if (n + 1 < N) o[1] = x.y;
+        if (n + 2 < N) o[2] = y.x;
+        if (n + 3 < N) o[3] = y.y;
+      }
     } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (n + i < N) o[i] = __float2bfloat16_rn(v[i]);
+      __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.out) + at;
+      if (vec) {
+        *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16(x.x, x.y), pack_bf16(y.x, y.y));
+      } else {
+        if (n < N) o[0] = __float2bfloat16_rn(x.x);
+        if (n + 1 < N) o[1] = __float2bfloat16_rn(x.y);
+        if (n + 2 < N) o[2] = __float2bfloat16_rn(y.x);
+        if (n + 3 < N) o[3] = __float2bfloat16_rn(y.y);
+      }
     }
   }
 }
 
-template <int BN>
+template <int BN, int ACT, int OUT>
 __global__ void __launch_bounds__(nk::THREADS)
     gemm_block_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ CUtensorMap tmQ,
                       const BlockGemmArgs a) {
@@ -138,7 +139,6 @@ __global__ void __launch_bounds__(nk::THREADS)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
-
   if (warp == 0) {
     if (lane == 0) {
       uint32_t used = 0, last_par = 0;
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(nk::THREADS)
       volatile int no_abort = 0;
       mbar_wait(done, 0, &no_abort, nullptr, DEV_TIMEOUT_DRAIN);
     }
-  } else {
+  } else if (warp < 6) {
     const int q = warp & 3;   // lane quarter of Tensor Memory
     const uint32_t quarter = tmem + ((uint32_t)(q * 32) << 16);
     bool ok = true;
@@ -234,30 +234,43 @@ __global__ void __launch_bounds__(nk::THREADS)
     if (!ok) *abort_flag = 1;
   }
   tc_fence_before();
-  __syncthreads();   // the partial accumulator is staged
-  if (splits > 1) cluster_sync();
-  if (!*abort_flag) {
-    const int n = n0 + lane * 4;
+  const int n = n0 + lane * 4;   // this lane's columns of C; their bias arrives during the barrier
+  unsigned short bias_bits[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (a.bias && n + i < a.N) bias_bits[i] = __ldg(reinterpret_cast<const unsigned short*>(a.bias) + n + i);
+  if (splits > 1)
+    cluster_sync();   // every rank's partial is staged
+  else
+    __syncthreads();
+  if (__all_sync(0xffffffffu, !*abort_flag)) {
     float bias[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) bias[i] = a.bias && n + i < a.N ? __bfloat162float(a.bias[n + i]) : 0.f;
-    for (int r = warp * splits + rank; r < BN && m0 + r < a.M; r += nk::THREADS / 32 * splits) {
-      const float* at = reinterpret_cast<const float*>(smem) + r * 128 + lane * 4;
-      float v[4];
-      if (splits == 1) {
-        const float4 u = *reinterpret_cast<const float4*>(at);
-        v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
-      } else {
+    for (int i = 0; i < 4; ++i) bias[i] = __uint_as_float((uint32_t)bias_bits[i] << 16);
+    const bool vec = a.N % 4 == 0 && n < a.N;   // four columns at an address aligned to them
+    const float* st = reinterpret_cast<const float*>(smem) + lane * 4;
+    const int rows = min(BN, a.M - m0);
+    constexpr int WARPS = nk::THREADS / 32;
+    if (splits == 1) {
+      for (int r = warp; r < rows; r += 4 * WARPS) {   // four rows at a time, for as many loads in flight
+        float4 u[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[i] = *reinterpret_cast<const float4*>(st + min(r + i * WARPS, BN - 1) * 128);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (r + i * WARPS < rows) write_row4<ACT, OUT>(a, m0 + r + i * WARPS, n, u[i], bias, vec);
+      }
+    } else {
+      for (int r = warp * splits + rank; r < rows; r += WARPS * splits) {
         float4 u[nk::MAX_SPLITS];
 #pragma unroll
         for (int k = 0; k < nk::MAX_SPLITS; ++k)
-          if (k < splits) u[k] = ld_cluster4(mapa_cluster(at, (uint32_t)k));
-        v[0] = u[0].x, v[1] = u[0].y, v[2] = u[0].z, v[3] = u[0].w;
+          if (k < splits) u[k] = ld_cluster4(mapa_cluster(st + r * 128, (uint32_t)k));
 #pragma unroll
         for (int k = 1; k < nk::MAX_SPLITS; ++k)
-          if (k < splits) v[0] += u[k].x, v[1] += u[k].y, v[2] += u[k].z, v[3] += u[k].w;
+          if (k < splits) u[0].x += u[k].x, u[0].y += u[k].y, u[0].z += u[k].z, u[0].w += u[k].w;
+        write_row4<ACT, OUT>(a, m0 + r, n, u[0], bias, vec);
       }
-      write_row4(a, m0 + r, n, v, bias);
     }
   }
   if (splits > 1) cluster_sync();   // no CTA leaves while another reads its partial
@@ -275,8 +288,6 @@ int launch_nk(const void* A8, const void* B8, const BlockGemmArgs& a, cudaStream
   int rc = make_tmap_2d(&tp, B8, 1, a.N, a.K, a.K, 128, 128, true);
   if (!rc) rc = make_tmap_2d(&tq, A8, 1, a.M, a.K, a.K, BN, 128, true);
   if (rc) return rc;
-  if (cudaFuncSetAttribute(gemm_block_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
-    return FW_ECUDA;
   const dim3 grid((a.N + 127) / 128 * a.splits, (a.M + BN - 1) / BN);
   if (grid.y > 65535) return FW_ESHAPE;
   cudaLaunchConfig_t cfg = {};
@@ -297,18 +308,36 @@ int launch_nk(const void* A8, const void* B8, const BlockGemmArgs& a, cudaStream
     attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
     ++cfg.numAttrs;
   }
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_block_kernel<BN>, tp, tq, a);
-  note_launch();
-  return e == cudaSuccess ? FW_OK : FW_ECUDA;
+  auto go = [&](auto kern) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return FW_ECUDA;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tp, tq, a);
+    note_launch();
+    return e == cudaSuccess ? FW_OK : FW_ECUDA;
+  };
+  auto by_act = [&](auto out) {
+    constexpr int O = decltype(out)::value;
+    switch (a.act) {
+      case ACT_TANH: return go(gemm_block_kernel<BN, ACT_TANH, O>);
+      case ACT_ERF: return go(gemm_block_kernel<BN, ACT_ERF, O>);
+      default: return go(gemm_block_kernel<BN, ACT_NONE, O>);
+    }
+  };
+  switch (a.out_dtype) {
+    case FW_U8: return by_act(std::integral_constant<int, FW_U8>{});
+    case FW_F32: return by_act(std::integral_constant<int, FW_F32>{});
+    default: return by_act(std::integral_constant<int, FW_BF16>{});
+  }
 }
 
 // Which kernel, tile and split: the least of a time model (us) whose constants were fitted to 70 measured
-// sizes (1 to 4000 rows, 30 to 13824 columns, 60 to 8960 of K): its choice is 3 % off the best variant on
-// average.  Small tiles: launch, then the busiest SM's operand bytes, or the latency of a CTA's chain of
-// k-blocks, or HBM, then the exposed epilogue and the join of a split; wide kernel: waves of 256 x 256 tiles.
+// sizes (1 to 4000 rows, 30 to 13824 columns, 60 to 8960 of K): its choice is 2 % off the best variant on average,
+// 30 % at worst.  Small tiles: launch, then the busiest SM's operand bytes, or the latency of a CTA's chain
+// of k-blocks, or HBM, then the exposed epilogue and the join of a split; wide kernel: waves of 256 x 256 tiles.
 // Both sides, measured: 880 x 1536 x 8960 18.4 us on 128-row tiles split 3 ways, 31.2 us wide; 2640 x 1536 x 1536
-// 14.1 and 11.0 us; 512 x 1536 x 4096 11.8 us split 5 ways, 19.3 us unsplit, 17.9 us wide; 1 x 9216 x 1536 6.8 us
-// split 4 ways, 7.3 us unsplit.  A split's CTAs are at most two per SM: more would wait for whole tiles to end.
+// 14.1 and 11.0 us; 512 x 1536 x 4096 12.2 us split 5 ways, 16.0 us unsplit, 17.9 us wide; 1 x 9216 x 1536 6.9 us
+// split 4 ways, 6.7 us unsplit; 1 x 1536 x 1536 4.7 us split 6 ways, 6.3 us unsplit.  A split's CTAs fill at most
+// 9/10 of two per SM: clusters do not fit every SM of a GPC, and what is left over waits for whole tiles to end
+// (512 x 1536 x 4096 on 64-row tiles split 3 ways, 288 CTAs: 18.6 us).
 struct Plan {
   int bn, splits;   // bn 0: the wide kernel
 };
@@ -319,16 +348,16 @@ Plan make_plan(int M, int N, int num_kb, int out_dtype) {
   const long long waves = up(up(M, 256) * up(N, 256), sms / 2);
   const bool tma_out = out_dtype == FW_U8 || N % (out_dtype == FW_F32 ? 4 : 8) == 0;
   Plan best = {0, 1};
-  double least = 4.0 + waves * (num_kb * 0.6 + (tma_out ? 1.0 : 3.5)) - 1.0;
+  double least = 5.7 + waves * (num_kb * 0.3 + (tma_out ? 1.0 : 3.5));
   for (int bn = 16; bn <= 128; bn *= 2) {
     if (up(M, bn) > 65535) continue;
     const long long tiles = up(N, 128) * up(M, bn);
     for (int sp = 1; sp <= nk::MAX_SPLITS && sp <= num_kb; ++sp) {
-      if (sp > 1 && tiles * sp > 2 * sms) break;
+      if (sp > 1 && tiles * sp > sms * 9 / 5) break;
       const double per_sm = (double)up(tiles * sp, sms), kbs = (double)up(num_kb, sp);
-      const double load = per_sm * kbs * (128 + bn) * b8::BLK / 6.0e4;
-      const double chain = up(tiles * sp, 2 * sms) * kbs * 0.18;
-      const double t = 3.0 + fmax(fmax(load, chain), hbm) + 1.1 * bn / 128 * per_sm + (sp > 1 ? 0.9 : 0.0);
+      const double load = per_sm * kbs * (128 + bn) * b8::BLK / 1.8e5;
+      const double chain = up(tiles * sp, 2 * sms) * kbs * 0.5;
+      const double t = 1.7 + fmax(fmax(load, chain), hbm) + 0.9 * bn / 128 * per_sm + (sp > 1 ? 3.4 : 0.0);
       if (t < least) {
         least = t;
         best = {bn, sp};
