@@ -8,52 +8,57 @@ namespace fw {
 
 namespace {
 
-// Four consecutive elements as fp32; VEC: the address is aligned to four elements and all are there.
-template <typename T> struct Load4;
-template <> struct Load4<float> {
-  static __device__ __forceinline__ void vec(const float* p, float (&v)[4]) {
-    const float4 u = *reinterpret_cast<const float4*>(p);
-    v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
+// Four consecutive columns of a row as loaded; VEC: one access, at an address aligned to it.
+template <typename T, bool VEC>
+struct Four {
+  float v[4];
+  __device__ __forceinline__ void load(const T* row, int c, int K) {   // columns [c, c + 4), zeros behind K
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = c + i < K ? static_cast<float>(row[c + i]) : 0.f;
   }
-  static __device__ __forceinline__ float one(float x) { return x; }
+  __device__ __forceinline__ void get(float (&o)[4]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = v[i];
+  }
 };
-template <> struct Load4<__nv_bfloat16> {
-  static __device__ __forceinline__ void vec(const __nv_bfloat16* p, float (&v)[4]) {
-    const uint2 u = *reinterpret_cast<const uint2*>(p);
+template <>
+struct Four<float, true> {
+  float4 u;
+  __device__ __forceinline__ void load(const float* row, int c, int K) {
+    u = c < K ? *reinterpret_cast<const float4*>(row + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  __device__ __forceinline__ void get(float (&o)[4]) const { o[0] = u.x, o[1] = u.y, o[2] = u.z, o[3] = u.w; }
+};
+template <>
+struct Four<__nv_bfloat16, true> {
+  uint2 u;
+  __device__ __forceinline__ void load(const __nv_bfloat16* row, int c, int K) {
+    u = c < K ? *reinterpret_cast<const uint2*>(row + c) : make_uint2(0u, 0u);
+  }
+  __device__ __forceinline__ void get(float (&o)[4]) const {
     const float2 a = unpack_bf16(u.x), b = unpack_bf16(u.y);
-    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+    o[0] = a.x, o[1] = a.y, o[2] = b.x, o[3] = b.y;
   }
-  static __device__ __forceinline__ float one(__nv_bfloat16 x) { return __bfloat162float(x); }
 };
-template <> struct Load4<__half> {
-  static __device__ __forceinline__ void vec(const __half* p, float (&v)[4]) {
-    const uint2 u = *reinterpret_cast<const uint2*>(p);
+template <>
+struct Four<__half, true> {
+  uint2 u;
+  __device__ __forceinline__ void load(const __half* row, int c, int K) {
+    u = c < K ? *reinterpret_cast<const uint2*>(row + c) : make_uint2(0u, 0u);
+  }
+  __device__ __forceinline__ void get(float (&o)[4]) const {
     const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
     const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
-    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+    o[0] = a.x, o[1] = a.y, o[2] = b.x, o[3] = b.y;
   }
-  static __device__ __forceinline__ float one(__half x) { return __half2float(x); }
 };
-// Columns [c, c + 4) of a row of K, zeros behind K.
-template <bool VEC, typename T>
-__device__ __forceinline__ void load4(const T* row, int c, int K, float (&v)[4]) {
-  if (VEC) {
-    if (c < K) {
-      Load4<T>::vec(row + c, v);
-    } else {
-      v[0] = v[1] = v[2] = v[3] = 0.f;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = c + i < K ? Load4<T>::one(row[c + i]) : 0.f;
-  }
-}
 
 // ---------------------------------------------------------------- quantiser
 // A warp takes one row's group of 512 columns: four blocks, four columns per lane and block, so
 // each load and each store of codes is contiguous over the warp and a block's maximum is one warp
-// reduction.  The eight warps of a CTA take eight neighbouring rows of one group, whose words of exponents are
-// one 32-byte sector.
+// reduction.  The eight warps of a CTA take eight neighbouring rows, whose words of exponents are one 32-byte
+// sector.  Many short CTAs keep HBM busiest: 2640 x 8960 bf16 in 13.2 us (5.4 TB/s); warps that took two,
+// three or six groups with the next one's loads in flight took 16.0, 16.2 and 17.3 us.
 constexpr int QROWS = 8;
 
 template <typename T, bool VEC>
@@ -61,23 +66,22 @@ __global__ void __launch_bounds__(QROWS * 32) quant_block_kernel(const T* __rest
                                                                  uint8_t* __restrict__ q, uint32_t* __restrict__ s) {
   pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int g = blockIdx.y;
+  const int lane = threadIdx.x & 31, g = blockIdx.y;
   const long long row = (long long)blockIdx.x * QROWS + (threadIdx.x >> 5);
   if (row >= M) return;
   const int Kp = b8::padded(K), c0 = g * b8::GRP * b8::BLK + lane * 4;
-  const T* src = x + (size_t)row * K;
-  float v[b8::GRP][4];
+  Four<T, VEC> in[b8::GRP];
 #pragma unroll
-  for (int b = 0; b < b8::GRP; ++b) load4<VEC>(src, c0 + b * b8::BLK, K, v[b]);
+  for (int b = 0; b < b8::GRP; ++b) in[b].load(x + (size_t)row * K, c0 + b * b8::BLK, K);
   uint32_t word = b8::ONES;
 #pragma unroll
   for (int b = 0; b < b8::GRP; ++b) {
     const int c = c0 + b * b8::BLK;
     if (c < Kp) {   // the same for the whole warp: Kp is a multiple of 128
+      float v[4];
+      in[b].get(v);
       uint32_t eb;
-      const uint32_t code = b8::encode_block(v[b], eb);
-      *reinterpret_cast<uint32_t*>(q + (size_t)row * Kp + c) = code;
+      *reinterpret_cast<uint32_t*>(q + (size_t)row * Kp + c) = b8::encode_block(v, eb);
       word = (word & ~(0xffu << (8 * b))) | (eb << (8 * b));
     }
   }
@@ -109,8 +113,20 @@ struct NormArgs {
   uint8_t* out_s;                                 // exponents of codes, null: bf16
 };
 
+// Columns [c, c + 4) of a row of K as fp32, zeros behind K.
+template <bool VEC, typename T>
+__device__ __forceinline__ void load4(const T* row, int c, int K, float (&v)[4]) {
+  Four<T, VEC> f;
+  f.load(row, c, K);
+  f.get(v);
+}
+
 // One row per CTA of W warps; warp w holds blocks [w NB, w NB + NB) of 128 columns in
-// registers, four columns per lane and block.
+// registers, four columns per lane and block.  HBM bounds it (12 bytes per element in bf16), but a row's bytes wait
+// behind up to four sums over the row, so many rows have to be in flight: 2640 x 1536 in 11.0 us (4.4 TB/s),
+// 6032 x 1536 in 20.9 us (5.3 TB/s), 4680 x 5120 in 66.8 us (4.3 TB/s).  Slower: CTAs that take several rows,
+// the next one's loads in flight (16.8 us at 2640 x 1536), and rows brought to a ring in shared memory by bulk copies
+// with a warp or four per row (27 us): fewer warps per SM are left to work through the sums.
 template <int W>
 __device__ __forceinline__ float row_sum(float v, float* slot, int warp, int lane) {
 #pragma unroll
@@ -160,33 +176,55 @@ __global__ void __launch_bounds__(W * 32) norm_gate_resid_kernel(const NormArgs 
   const int b0 = warp * NB, c0 = b0 * b8::BLK + lane * 4;
   const size_t frame = (size_t)(row / a.rows_per_frame) * D;
   float* xr = a.resid + (size_t)row * D;
-  float x[NB][4];
+  // A parameter's loads for all blocks are issued together, several parameters' before one is used: with
+  // one block after the other, each waited for its own.  The branch's parameters are asked for before the first
+  // sum, the output's after the last one (earlier, their registers would cost rows in flight).
+  Four<__nv_bfloat16, VEC> w[NB];
+  Four<float, VEC> f[NB], f2[NB];
+  auto fetch = [&](auto& v, const auto* base) {
 #pragma unroll
-  for (int b = 0; b < NB; ++b) load4<VEC>(xr, c0 + b * b8::BLK, D, x[b]);
+    for (int b = 0; b < NB; ++b) v[b].load(base, c0 + b * b8::BLK, D);
+  };
+  auto mul = [&](float (&v)[NB][4], auto& by) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      float p[4];
+      by[b].get(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[b][i] *= p[i];
+    }
+  };
+  auto add = [&](float (&v)[NB][4], auto& by) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      float p[4];
+      by[b].get(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[b][i] += p[i];
+    }
+  };
+  Four<float, VEC> xin[NB];
+  fetch(xin, xr);
+  float x[NB][4];
   if (a.y) {
+    Four<Y, VEC> yin[NB];
+    fetch(yin, static_cast<const Y*>(a.y) + (size_t)row * D);
+    if (a.post_w) fetch(w, a.post_w);
+    if (a.gate) fetch(f, a.gate + frame);
     float y[NB][4];
 #pragma unroll
-    for (int b = 0; b < NB; ++b) load4<VEC>(static_cast<const Y*>(a.y) + (size_t)row * D, c0 + b * b8::BLK, D, y[b]);
+    for (int b = 0; b < NB; ++b) yin[b].get(y[b]);
     if (a.post != FW_NORM_NONE) norm_row<W, NB>(y, a.post, a.eps, D, c0, slots, warp, lane);
+    if (a.post_w) mul(y, w);
+    if (a.post_b) {
+      fetch(w, a.post_b);
+      add(y, w);
+    }
+    if (a.gate) mul(y, f);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       const int c = c0 + b * b8::BLK;
-      float p[4];
-      if (a.post_w) {
-        load4<VEC>(a.post_w, c, D, p);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y[b][i] *= p[i];
-      }
-      if (a.post_b) {
-        load4<VEC>(a.post_b, c, D, p);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y[b][i] += p[i];
-      }
-      if (a.gate) {
-        load4<VEC>(a.gate + frame, c, D, p);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y[b][i] *= p[i];
-      }
+      xin[b].get(x[b]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[b][i] = a.resid_scale * x[b][i] + a.branch_scale * y[b][i];
       if (VEC) {
@@ -197,32 +235,36 @@ __global__ void __launch_bounds__(W * 32) norm_gate_resid_kernel(const NormArgs 
           if (c + i < D) xr[c + i] = x[b][i];
       }
     }
+  } else {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) xin[b].get(x[b]);
   }
   if (!a.out) return;
   if (a.pre != FW_NORM_NONE) norm_row<W, NB>(x, a.pre, a.eps, D, c0, slots + 2 * W, warp, lane);
+  if (a.pre_w) fetch(w, a.pre_w);
+  if (a.scale) {
+    fetch(f, a.scale + frame);
+    fetch(f2, a.shift + frame);
+  }
+  if (a.pre_w) mul(x, w);
+  if (a.pre_b) {
+    fetch(w, a.pre_b);
+    add(x, w);
+  }
+  if (a.scale) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      float p[4], t[4];
+      f[b].get(p);
+      f2[b].get(t);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[b][i] = x[b][i] * (1.f + p[i]) + t[i];
+    }
+  }
   const int Dp = b8::padded(D);
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     const int c = c0 + b * b8::BLK;
-    float p[4];
-    if (a.pre_w) {
-      load4<VEC>(a.pre_w, c, D, p);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[b][i] *= p[i];
-    }
-    if (a.pre_b) {
-      load4<VEC>(a.pre_b, c, D, p);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[b][i] += p[i];
-    }
-    if (a.scale) {
-      load4<VEC>(a.scale + frame, c, D, p);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[b][i] *= 1.f + p[i];
-      load4<VEC>(a.shift + frame, c, D, p);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[b][i] += p[i];
-    }
     if (a.out_s) {
       const int blk = b0 + b;
       if (blk * b8::BLK < Dp) {   // zeros behind D: every parameter reads as zero there
@@ -246,6 +288,8 @@ __global__ void __launch_bounds__(W * 32) norm_gate_resid_kernel(const NormArgs 
       a.out_s[((size_t)(blk / b8::GRP) * a.M + row) * b8::GRP + blk % b8::GRP] = 127;
 }
 
+// Warps per row and blocks per warp by the row's width: at 1536 columns 4 x 3 measured 11.1 us for 2640 rows, 6 x 2
+// 12.2, 12 x 1 16.1 and 2 x 6 12.1; at 5120 columns 10 x 4 66.8 us for 4680 rows, 14 x 3 65.9, 8 x 6 68.4, 20 x 2 105.
 template <typename Y, bool VEC>
 int norm_launch(const NormArgs& a, cudaStream_t s) {
   const int nb = b8::blocks(a.D);
@@ -254,7 +298,9 @@ int norm_launch(const NormArgs& a, cudaStream_t s) {
   };
   if (nb <= 4) return go(norm_gate_resid_kernel<Y, VEC, 4, 1>, 4);
   if (nb <= 12) return go(norm_gate_resid_kernel<Y, VEC, 4, 3>, 4);
-  if (nb <= 48) return go(norm_gate_resid_kernel<Y, VEC, 8, 6>, 8);
+  if (nb <= 24) return go(norm_gate_resid_kernel<Y, VEC, 8, 3>, 8);
+  if (nb <= 40) return go(norm_gate_resid_kernel<Y, VEC, 10, 4>, 10);
+  if (nb <= 64) return go(norm_gate_resid_kernel<Y, VEC, 16, 4>, 16);
   return go(norm_gate_resid_kernel<Y, VEC, 16, 8>, 16);
 }
 

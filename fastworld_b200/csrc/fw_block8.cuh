@@ -17,6 +17,36 @@
 #include "fw_ptx.cuh"
 
 namespace fw {
+
+// Bounded wait for a phase, for loops whose issue rate counts: one try that lets the hardware hold
+// the thread until the phase completes (up to a millisecond), and everything else out of line, so
+// that little code sits between two MMAs.
+__device__ __forceinline__ bool mbar_try_held(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
+      : "memory");
+  return ok != 0;
+}
+static __device__ __noinline__ bool wait_again(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  const uint64_t t0 = globaltimer();
+  for (;;) {
+    if (mbar_try_held(bar, parity)) return true;
+    if (*abort) return false;
+    if (globaltimer() - t0 > FW_WAIT_LIMIT_NS) {
+      *abort = 1;
+      return false;
+    }
+  }
+}
+__device__ __forceinline__ bool wait_on(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  return mbar_try_held(bar, parity) || wait_again(bar, parity, abort);
+}
+
 namespace b8 {
 
 constexpr int BLK = 128;            // columns that share a scale
@@ -62,8 +92,15 @@ __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, 
 }
 // One block across a warp, four consecutive columns per lane: codes of this lane, exponent byte.
 __device__ __forceinline__ uint32_t encode_block(const float (&v)[4], uint32_t& eb) {
-  const uint32_t m = max(max(abs_bits(v[0]), abs_bits(v[1])), max(abs_bits(v[2]), abs_bits(v[3])));
-  eb = block_exp(__reduce_max_sync(0xffffffffu, m));
+  // the largest magnitude, passing over NaN; only an infinity needs the look at every element
+  const float top = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+  const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+  if (m < 0x7f800000u) {
+    eb = block_exp(m);
+    return encode4_finite(v[0], v[1], v[2], v[3], inv_scale(eb));
+  }
+  const uint32_t f = max(max(abs_bits(v[0]), abs_bits(v[1])), max(abs_bits(v[2]), abs_bits(v[3])));
+  eb = block_exp(__reduce_max_sync(0xffffffffu, f));
   return encode4(v[0], v[1], v[2], v[3], inv_scale(eb));
 }
 

@@ -18,35 +18,6 @@ struct BlockGemmArgs {
   uint8_t* out_s;              // exponents of codes
 };
 
-// Bounded wait for a phase, for loops whose issue rate counts: one try that lets the hardware hold
-// the thread until the phase completes (up to a millisecond), and everything else out of line, so
-// that little code sits between two MMAs.
-__device__ __forceinline__ bool mbar_try_held(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
-      : "memory");
-  return ok != 0;
-}
-static __device__ __noinline__ bool wait_again(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  const uint64_t t0 = globaltimer();
-  for (;;) {
-    if (mbar_try_held(bar, parity)) return true;
-    if (*abort) return false;
-    if (globaltimer() - t0 > FW_WAIT_LIMIT_NS) {
-      *abort = 1;
-      return false;
-    }
-  }
-}
-__device__ __forceinline__ bool wait_on(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  return mbar_try_held(bar, parity) || wait_again(bar, parity, abort);
-}
-
 // Instruction descriptor of kind::mxf8f6f4: e4m3 operands, both K-major, UE8M0 scales (bit 23).
 __host__ __device__ constexpr uint32_t idesc_mx8(int M, int N) {
   return ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((uint32_t)(M >> 4) << 24);
