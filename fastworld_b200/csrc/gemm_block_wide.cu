@@ -154,9 +154,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
       const uint32_t sf_smem = smem_u32(smem + SF_OFF);
       bool ok = true;
       for (int t = pair; t < num_tiles && ok; t += npairs, ++it) {
-        // tile it - 1's shared columns have been read, and all of tile it - 2
-        if (it > 0 && !wait_on(tfree, (it - 1) & 1u, abort_flag)) break;
-        tc_fence_after();
         const uint32_t d = tmem + (it & 1u) * SHIFT;
         uint32_t accumulate = 0;
         for (int left = num_kb; left > 0;) {
@@ -166,6 +163,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
 #pragma unroll
           for (int c = 0; c < 3; ++c) tmem_copy_if<2>(one, sf + 4 * c, sf_smem + slot * SF_BYTES + 512 * c);
           uint32_t id = idesc_mx8(BM, BN);
+          // a tile's first MMA: tile it - 1's shared columns have been read, and all of tile it - 2
+          if (!accumulate && it > 0) ok = wait_on(tfree, (it - 1) & 1u, abort_flag);
+          if (!ok) break;
           const int n = min(left, b8::GRP);
           for (int k = 0; k < n; ++k) {
             ok = wait_on(full + stage, phase, abort_flag);

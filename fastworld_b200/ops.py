@@ -215,6 +215,19 @@ def gemm_e4m3_block(a8: torch.Tensor, sa: torch.Tensor, b8: torch.Tensor, sb: to
     return o if so is None else (o, so)
 
 
+def _weight(name, t, D, index):
+    if t.dtype is not torch.bfloat16 or t.shape != (D,) or t.get_device() != index or not t.is_contiguous():
+        _refuse(name, t, torch.bfloat16, index, [D])
+
+
+def _per_frame(name, t, frames, D, index):
+    """fp32 [at least frames, D], or [D] for one frame."""
+    shape = t.shape
+    if (t.dtype is not torch.float32 or shape[-1:] != (D,) or t.get_device() != index or not t.is_contiguous()
+            or not (len(shape) == 2 and shape[0] >= frames or len(shape) == 1 and frames <= 1)):
+        _refuse(name, t, torch.float32, index, f"[{frames}, {D}]" + (f" or [{D}]" if frames <= 1 else ""))
+
+
 def norm_gate_resid_(resid: torch.Tensor, y=None, post=None, post_w=None, post_b=None, gate=None,
                      resid_scale: float = 1.0, branch_scale: float = 1.0, pre="layer", pre_w=None, pre_b=None,
                      shift=None, scale=None, rows_per_frame=None, eps: float = 1e-6, out="bf16"):
@@ -228,43 +241,50 @@ def norm_gate_resid_(resid: torch.Tensor, y=None, post=None, post_w=None, post_b
     f = row // rows_per_frame (None: all rows are one frame).  out: 'bf16', 'e4m3' (the pair (q, s) of
     quant_e4m3_block, quantised from fp32) or None (h is not computed)."""
     f32, b16, index, shape = torch.float32, torch.bfloat16, resid.get_device(), resid.shape
-    if index < 0 or len(shape) != 2 or shape[1] == 0 or not _is(resid, f32, index):
+    if index < 0 or len(shape) != 2 or shape[1] == 0 or resid.dtype is not f32 or not resid.is_contiguous():
         _refuse("resid", resid, f32, index, "[M, D > 0]")
     M, D = shape
     if post not in NORMS or pre not in NORMS:
         raise ValueError(f"post, pre: {post!r}, {pre!r}, expected 'layer', 'rms' or None")
     if out not in ("bf16", "e4m3", None):
         raise ValueError(f"out: {out!r}, expected 'bf16', 'e4m3' or None")
-    if y is None and out is None:
-        raise ValueError("nothing to do: no y and no output")
-    if y is None and not (post is None and post_w is None and post_b is None and gate is None and resid_scale == 1.0
-                          and branch_scale == 1.0):
-        raise ValueError("post, post_w, post_b, gate, resid_scale and branch_scale need y")
+    rpf = (M or 1) if rows_per_frame is None else int(rows_per_frame)
+    if rpf <= 0:
+        raise ValueError(f"rows_per_frame: {rows_per_frame}")
+    frames = -(-M // rpf)
+    if y is None:
+        if out is None:
+            raise ValueError("nothing to do: no y and no output")
+        if not (post is None and post_w is None and post_b is None and gate is None and resid_scale == 1.0
+                and branch_scale == 1.0):
+            raise ValueError("post, post_w, post_b, gate, resid_scale and branch_scale need y")
+    else:
+        if (y.dtype is not b16 and y.dtype is not f32) or y.shape != shape or y.get_device() != index or not y.is_contiguous():
+            _refuse("y", y, "bf16 or fp32", index, [M, D])
+        if post_w is not None:
+            _weight("post_w", post_w, D, index)
+        if post_b is not None:
+            _weight("post_b", post_b, D, index)
+        if gate is not None:
+            _per_frame("gate", gate, frames, D, index)
     if out is None and not (pre_w is None and pre_b is None and shift is None and scale is None):
         raise ValueError("pre_w, pre_b, shift and scale need an output")
     if (shift is None) != (scale is None):
         raise ValueError("shift and scale come together")
-    rpf = max(M, 1) if rows_per_frame is None else int(rows_per_frame)
-    if rpf <= 0:
-        raise ValueError(f"rows_per_frame: {rows_per_frame}")
-    if y is not None and (y.dtype not in (b16, f32) or y.shape != shape or not _is(y, y.dtype, index)):
-        _refuse("y", y, "bf16 or fp32", index, [M, D])
-    for n, t in (("post_w", post_w), ("post_b", post_b), ("pre_w", pre_w), ("pre_b", pre_b)):
-        if t is not None and (t.shape != (D,) or not _is(t, b16, index)):
-            _refuse(n, t, b16, index, [D])
-    frames = -(-M // rpf)
-    for n, t in (("gate", gate), ("shift", shift), ("scale", scale)):
-        if t is not None:
-            ts = t.shape
-            if not (len(ts) == 2 and ts[0] >= frames or len(ts) == 1 and frames <= 1) or ts[-1] != D or not _is(t, f32, index):
-                _refuse(n, t, f32, index, f"[{frames}, {D}]" + (f" or [{D}]" if frames <= 1 else ""))
+    if shift is not None:
+        _per_frame("shift", shift, frames, D, index)
+        _per_frame("scale", scale, frames, D, index)
+    if pre_w is not None:
+        _weight("pre_w", pre_w, D, index)
+    if pre_b is not None:
+        _weight("pre_b", pre_b, D, index)
     h = s = None
     if out == "e4m3":
         h, s = _block_empty(M, D, resid.device)
     elif out == "bf16":
         h = torch.empty(M, D, device=resid.device, dtype=torch.bfloat16)
-    a = _lib.FwNormArgs(resid.data_ptr(), ptr(y), _lib.DT_BF16 if y is None else _DTYPES[y.dtype], NORMS[post], NORMS[pre],
-                        ptr(post_w), ptr(post_b), ptr(pre_w), ptr(pre_b), ptr(gate), ptr(shift), ptr(scale),
-                        resid_scale, branch_scale, eps, M, D, min(rpf, 2**31 - 1), ptr(h), ptr(s))
+    a = _lib.FwNormArgs(resid.data_ptr(), ptr(y), _lib.DT_F32 if y is not None and y.dtype is f32 else _lib.DT_BF16,
+                        NORMS[post], NORMS[pre], ptr(post_w), ptr(post_b), ptr(pre_w), ptr(pre_b), ptr(gate), ptr(shift),
+                        ptr(scale), resid_scale, branch_scale, eps, M, D, min(rpf, 2**31 - 1), ptr(h), ptr(s))
     _on(index, lib().fw_norm_gate_resid, "norm_gate_resid", ctypes.byref(a))
     return (h, s) if out == "e4m3" else h
