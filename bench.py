@@ -580,7 +580,7 @@ def tp_parity_variant(rank, world, local, ctl):
 
 # ---------------------------------------------------------------- single-kernel workloads
 # Small, self-terminating runs of one kernel for ncu captures and CUDA-event timing:
-#   python bench.py --kernel gemm|gemm_resid|attn|ln|ln14|rms|copy|fp8_peak [--reps 3]
+#   python bench.py --kernel gemm|gemm_resid|attn|ln|ln14|rms|copy|block8|fp8_peak [--reps 3]
 #   python bench.py --kernel chunk [--chunks 2] [--config mg2|mg2_fp8]   (eager chunks)
 
 def chunk(n: int, config: str = "mg2") -> None:
@@ -817,6 +817,49 @@ def copy(reps: int) -> None:
     print(f"copy_kernel 649 MB: {ms * 1e3:.1f} us, {2 * nb / ms / 1e6:.0f} GB/s (read + write)")
 
 
+def block8(reps: int) -> None:
+    """Block-scaled e4m3 operators at the MG2 and 14B widths: quantise, product, norm, each over operand sets
+    larger than L2."""
+    from fastworld_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(0)
+
+    def rand(*shape, dtype=torch.bfloat16, size=1.0):
+        return (torch.randn(*shape, device="cuda", generator=g) * size).to(dtype)
+
+    def run(name, fns, work, unit):
+        for _ in range(reps):
+            for f in fns:
+                f()
+        torch.cuda.synchronize()
+        held = []   # the recorded pass's results stay allocated while it is replayed
+
+        def first():
+            held.clear()
+            held.append(fns[0]())
+        ms = _graph_ms([first] + [lambda f=f: held.append(f()) for f in fns[1:]])
+        print(f"{name}: {ms * 1e3:.2f} us/launch, {work / ms / 1e9:.0f} {unit}" if unit == "TFLOP/s" else
+              f"{name}: {ms * 1e3:.2f} us/launch, {work / ms / 1e6:.0f} {unit}")
+
+    xs = _rows(6, lambda i: rand(2640, 8960))
+    run("quant_e4m3_block 2640x8960", [lambda x=x: ops.quant_e4m3_block(x) for x in xs], 2640 * 8960 * (3 + 1 / 128), "GB/s")
+    del xs
+    for M, N, K, epi, out in ((2640, 4608, 1536, "none", "bf16"), (2640, 8960, 1536, "gelu_tanh", "e4m3"),
+                              (2640, 1536, 8960, "none", "bf16"), (4680, 13824, 5120, "gelu_tanh", "bf16"),
+                              (512, 1536, 4096, "gelu_tanh", "bf16"), (1, 9216, 1536, "none", "f32")):
+        sets = _rows(max(2, min(24, int(2.6e8 / ((M + N) * K)) + 1)),
+                     lambda i: (*ops.quant_e4m3_block(rand(M, K)), *ops.quant_e4m3_block(rand(N, K, size=K ** -0.5)), rand(N)))
+        run(f"gemm_e4m3_block {M}x{N}x{K} {epi} {out}",
+            [lambda s=s: ops.gemm_e4m3_block(*s, epilogue=epi, out=out) for s in sets], 2.0 * M * N * K, "TFLOP/s")
+        del sets
+    for M, D in ((2640, 1536), (4680, 5120)):
+        w, (gate, shift, scale) = rand(D), (rand(3, D, dtype=torch.float32, size=0.3) for _ in range(3))
+        sets = _rows(8 if D == 1536 else 2, lambda i: (rand(M, D, dtype=torch.float32), rand(M, D)))
+        run(f"norm_gate_resid {M}x{D}",
+            [lambda s=s: ops.norm_gate_resid_(s[0], s[1], post="rms", post_w=w, gate=gate, pre="layer", shift=shift,
+                                              scale=scale, rows_per_frame=M // 3) for s in sets], M * D * 12, "GB/s")
+        del sets
+
+
 def taehv_decode_ms(replays: int = 10):
     """TinyVAE (taew2_1) on one MG2 latent chunk: warm graph replays timed with CUDA events.
     Returns (ms per chunk, the decoder) after checking the device status."""
@@ -870,7 +913,7 @@ KERNELS = {"chunk": lambda a: chunk(a.chunks, a.config), "gemm": lambda a: gemm(
            "lingbot": lambda a: lingbot(a.reps), "lingbot_chunk": lambda a: lingbot_chunk(a.reps),
            "gemm_resid": lambda a: gemm_resid(a.reps), "attn": lambda a: attn(a.reps), "ln": lambda a: ln(a.reps),
            "ln14": lambda a: ln14(a.reps), "rms": lambda a: rms(a.reps), "copy": lambda a: copy(a.reps),
-           "fp8_peak": lambda a: fp8_peak(a.reps), "gemm_vs_cublas": lambda a: gemm_vs_cublas(a.reps)}
+           "block8": lambda a: block8(a.reps), "fp8_peak": lambda a: fp8_peak(a.reps), "gemm_vs_cublas": lambda a: gemm_vs_cublas(a.reps)}
 
 
 def main():

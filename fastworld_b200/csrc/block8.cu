@@ -16,9 +16,9 @@ struct Four {
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = c + i < K ? static_cast<float>(row[c + i]) : 0.f;
   }
-  __device__ __forceinline__ void get(float (&o)[4]) const {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = v[i];
+  __device__ __forceinline__ void get(float2 (&o)[2]) const {
+    o[0] = make_float2(v[0], v[1]);
+    o[1] = make_float2(v[2], v[3]);
   }
 };
 template <>
@@ -27,7 +27,10 @@ struct Four<float, true> {
   __device__ __forceinline__ void load(const float* row, int c, int K) {
     u = c < K ? *reinterpret_cast<const float4*>(row + c) : make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  __device__ __forceinline__ void get(float (&o)[4]) const { o[0] = u.x, o[1] = u.y, o[2] = u.z, o[3] = u.w; }
+  __device__ __forceinline__ void get(float2 (&o)[2]) const {
+    o[0] = make_float2(u.x, u.y);
+    o[1] = make_float2(u.z, u.w);
+  }
 };
 template <>
 struct Four<__nv_bfloat16, true> {
@@ -35,9 +38,9 @@ struct Four<__nv_bfloat16, true> {
   __device__ __forceinline__ void load(const __nv_bfloat16* row, int c, int K) {
     u = c < K ? *reinterpret_cast<const uint2*>(row + c) : make_uint2(0u, 0u);
   }
-  __device__ __forceinline__ void get(float (&o)[4]) const {
-    const float2 a = unpack_bf16(u.x), b = unpack_bf16(u.y);
-    o[0] = a.x, o[1] = a.y, o[2] = b.x, o[3] = b.y;
+  __device__ __forceinline__ void get(float2 (&o)[2]) const {
+    o[0] = unpack_bf16(u.x);
+    o[1] = unpack_bf16(u.y);
   }
 };
 template <>
@@ -46,10 +49,9 @@ struct Four<__half, true> {
   __device__ __forceinline__ void load(const __half* row, int c, int K) {
     u = c < K ? *reinterpret_cast<const uint2*>(row + c) : make_uint2(0u, 0u);
   }
-  __device__ __forceinline__ void get(float (&o)[4]) const {
-    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
-    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
-    o[0] = a.x, o[1] = a.y, o[2] = b.x, o[3] = b.y;
+  __device__ __forceinline__ void get(float2 (&o)[2]) const {
+    o[0] = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
+    o[1] = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
   }
 };
 
@@ -78,7 +80,7 @@ __global__ void __launch_bounds__(QROWS * 32) quant_block_kernel(const T* __rest
   for (int b = 0; b < b8::GRP; ++b) {
     const int c = c0 + b * b8::BLK;
     if (c < Kp) {   // the same for the whole warp: Kp is a multiple of 128
-      float v[4];
+      float2 v[2];
       in[b].get(v);
       uint32_t eb;
       *reinterpret_cast<uint32_t*>(q + (size_t)row * Kp + c) = b8::encode_block(v, eb);
@@ -113,14 +115,6 @@ struct NormArgs {
   uint8_t* out_s;                                 // exponents of codes, null: bf16
 };
 
-// Columns [c, c + 4) of a row of K as fp32, zeros behind K.
-template <bool VEC, typename T>
-__device__ __forceinline__ void load4(const T* row, int c, int K, float (&v)[4]) {
-  Four<T, VEC> f;
-  f.load(row, c, K);
-  f.get(v);
-}
-
 // One row per CTA of W warps; warp w holds blocks [w NB, w NB + NB) of 128 columns in
 // registers, four columns per lane and block.  HBM bounds it (12 bytes per element in bf16), but a row's bytes wait
 // behind up to four sums over the row, so many rows have to be in flight: 2640 x 1536 in 11.0 us (4.4 TB/s),
@@ -140,30 +134,44 @@ __device__ __forceinline__ float row_sum(float v, float* slot, int warp, int lan
   return t;
 }
 
-// Normalises x in place: fp32 mean and, about it, fp32 mean square (two sums, no cancellation).
+// Normalises x in place: fp32 mean and, about it, fp32 mean square (two sums, no cancellation).  Pairs of
+// columns on the packed fp32 pipe: with few rows per SM in flight, instructions count as much as bytes.
 template <int W, int NB>
-__device__ __forceinline__ void norm_row(float (&x)[NB][4], int kind, float eps, int D, int c0, float* slots, int warp,
+__device__ __forceinline__ void norm_row(float2 (&x)[NB][2], int kind, float eps, int D, int c0, float* slots, int warp,
                                          int lane) {
   const float inv_d = 1.f / (float)D;
   if (kind == FW_NORM_LAYER) {
-    float t = 0.f;
+    float2 t = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int b = 0; b < NB; ++b) t += (x[b][0] + x[b][1]) + (x[b][2] + x[b][3]);   // zeros behind D
-    const float mu = row_sum<W>(t, slots, warp, lane) * inv_d;
+    for (int b = 0; b < NB; ++b) t = __fadd2_rn(t, __fadd2_rn(x[b][0], x[b][1]));   // zeros behind D
+    const float mu = row_sum<W>(t.x + t.y, slots, warp, lane) * inv_d;
+    const float2 m2 = make_float2(-mu, -mu);
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+    for (int b = 0; b < NB; ++b) {
+      x[b][0] = __fadd2_rn(x[b][0], m2);
+      x[b][1] = __fadd2_rn(x[b][1], m2);
+    }
+    if (D % (W * NB * b8::BLK) != 0) {   // zeros behind D again
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[b][i] = c0 + b * b8::BLK + i < D ? x[b][i] - mu : 0.f;
+      for (int b = 0; b < NB; ++b) {
+        const int c = c0 + b * b8::BLK;
+        if (c >= D) x[b][0].x = 0.f;
+        if (c + 1 >= D) x[b][0].y = 0.f;
+        if (c + 2 >= D) x[b][1].x = 0.f;
+        if (c + 3 >= D) x[b][1].y = 0.f;
+      }
+    }
   }
-  float t = 0.f;
+  float2 t = make_float2(0.f, 0.f);
 #pragma unroll
-  for (int b = 0; b < NB; ++b)
-    t += (x[b][0] * x[b][0] + x[b][1] * x[b][1]) + (x[b][2] * x[b][2] + x[b][3] * x[b][3]);
-  const float r = rsqrtf(row_sum<W>(t, slots + W, warp, lane) * inv_d + eps);
+  for (int b = 0; b < NB; ++b) t = __ffma2_rn(x[b][1], x[b][1], __ffma2_rn(x[b][0], x[b][0], t));
+  const float r = rsqrtf(row_sum<W>(t.x + t.y, slots + W, warp, lane) * inv_d + eps);
+  const float2 r2 = make_float2(r, r);
 #pragma unroll
-  for (int b = 0; b < NB; ++b)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[b][i] *= r;
+  for (int b = 0; b < NB; ++b) {
+    x[b][0] = __fmul2_rn(x[b][0], r2);
+    x[b][1] = __fmul2_rn(x[b][1], r2);
+  }
 }
 
 template <typename Y, bool VEC, int W, int NB>
@@ -185,33 +193,33 @@ __global__ void __launch_bounds__(W * 32) norm_gate_resid_kernel(const NormArgs 
 #pragma unroll
     for (int b = 0; b < NB; ++b) v[b].load(base, c0 + b * b8::BLK, D);
   };
-  auto mul = [&](float (&v)[NB][4], auto& by) {
+  auto mul = [&](float2 (&v)[NB][2], auto& by) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      float p[4];
+      float2 p[2];
       by[b].get(p);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[b][i] *= p[i];
+      v[b][0] = __fmul2_rn(v[b][0], p[0]);
+      v[b][1] = __fmul2_rn(v[b][1], p[1]);
     }
   };
-  auto add = [&](float (&v)[NB][4], auto& by) {
+  auto add = [&](float2 (&v)[NB][2], auto& by) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      float p[4];
+      float2 p[2];
       by[b].get(p);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[b][i] += p[i];
+      v[b][0] = __fadd2_rn(v[b][0], p[0]);
+      v[b][1] = __fadd2_rn(v[b][1], p[1]);
     }
   };
   Four<float, VEC> xin[NB];
   fetch(xin, xr);
-  float x[NB][4];
+  float2 x[NB][2];
   if (a.y) {
     Four<Y, VEC> yin[NB];
     fetch(yin, static_cast<const Y*>(a.y) + (size_t)row * D);
     if (a.post_w) fetch(w, a.post_w);
     if (a.gate) fetch(f, a.gate + frame);
-    float y[NB][4];
+    float2 y[NB][2];
 #pragma unroll
     for (int b = 0; b < NB; ++b) yin[b].get(y[b]);
     if (a.post != FW_NORM_NONE) norm_row<W, NB>(y, a.post, a.eps, D, c0, slots, warp, lane);
@@ -225,14 +233,16 @@ __global__ void __launch_bounds__(W * 32) norm_gate_resid_kernel(const NormArgs 
     for (int b = 0; b < NB; ++b) {
       const int c = c0 + b * b8::BLK;
       xin[b].get(x[b]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[b][i] = a.resid_scale * x[b][i] + a.branch_scale * y[b][i];
+      const float2 rs = make_float2(a.resid_scale, a.resid_scale), bs = make_float2(a.branch_scale, a.branch_scale);
+      x[b][0] = __ffma2_rn(bs, y[b][0], __fmul2_rn(rs, x[b][0]));
+      x[b][1] = __ffma2_rn(bs, y[b][1], __fmul2_rn(rs, x[b][1]));
       if (VEC) {
-        if (c < D) *reinterpret_cast<float4*>(xr + c) = make_float4(x[b][0], x[b][1], x[b][2], x[b][3]);
+        if (c < D) *reinterpret_cast<float4*>(xr + c) = make_float4(x[b][0].x, x[b][0].y, x[b][1].x, x[b][1].y);
       } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (c + i < D) xr[c + i] = x[b][i];
+        if (c < D) xr[c] = x[b][0].x;
+        if (c + 1 < D) xr[c + 1] = x[b][0].y;
+        if (c + 2 < D) xr[c + 2] = x[b][1].x;
+        if (c + 3 < D) xr[c + 3] = x[b][1].y;
       }
     }
   } else {
@@ -254,11 +264,11 @@ __global__ void __launch_bounds__(W * 32) norm_gate_resid_kernel(const NormArgs 
   if (a.scale) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      float p[4], t[4];
+      float2 p[2], t[2];
       f[b].get(p);
       f2[b].get(t);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[b][i] = x[b][i] * (1.f + p[i]) + t[i];
+      for (int i = 0; i < 2; ++i) x[b][i] = __ffma2_rn(x[b][i], p[i], __fadd2_rn(x[b][i], t[i]));   // x (1 + p) + t
     }
   }
   const int Dp = b8::padded(D);
@@ -276,11 +286,13 @@ __global__ void __launch_bounds__(W * 32) norm_gate_resid_kernel(const NormArgs 
     } else if (VEC) {
       if (c < D)
         *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + (size_t)row * D + c) =
-            make_uint2(pack_bf16(x[b][0], x[b][1]), pack_bf16(x[b][2], x[b][3]));
+            make_uint2(pack_bf16(x[b][0].x, x[b][0].y), pack_bf16(x[b][1].x, x[b][1].y));
     } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (c + i < D) static_cast<__nv_bfloat16*>(a.out)[(size_t)row * D + c + i] = __float2bfloat16_rn(x[b][i]);
+      __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.out) + (size_t)row * D;
+      if (c < D) o[c] = __float2bfloat16_rn(x[b][0].x);
+      if (c + 1 < D) o[c + 1] = __float2bfloat16_rn(x[b][0].y);
+      if (c + 2 < D) o[c + 2] = __float2bfloat16_rn(x[b][1].x);
+      if (c + 3 < D) o[c + 3] = __float2bfloat16_rn(x[b][1].y);
     }
   }
   if (a.out_s && threadIdx.x == 0)   // places behind the last block

@@ -91,17 +91,17 @@ __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, 
   return (uint32_t)lo | ((uint32_t)hi << 16);
 }
 // One block across a warp, four consecutive columns per lane: codes of this lane, exponent byte.
-__device__ __forceinline__ uint32_t encode_block(const float (&v)[4], uint32_t& eb) {
+__device__ __forceinline__ uint32_t encode_block(const float2 (&v)[2], uint32_t& eb) {
   // the largest magnitude, passing over NaN; only an infinity needs the look at every element
-  const float top = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+  const float top = fmaxf(fmaxf(fabsf(v[0].x), fabsf(v[0].y)), fmaxf(fabsf(v[1].x), fabsf(v[1].y)));
   const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
   if (m < 0x7f800000u) {
     eb = block_exp(m);
-    return encode4_finite(v[0], v[1], v[2], v[3], inv_scale(eb));
+    return encode4_finite(v[0].x, v[0].y, v[1].x, v[1].y, inv_scale(eb));
   }
-  const uint32_t f = max(max(abs_bits(v[0]), abs_bits(v[1])), max(abs_bits(v[2]), abs_bits(v[3])));
+  const uint32_t f = max(max(abs_bits(v[0].x), abs_bits(v[0].y)), max(abs_bits(v[1].x), abs_bits(v[1].y)));
   eb = block_exp(__reduce_max_sync(0xffffffffu, f));
-  return encode4(v[0], v[1], v[2], v[3], inv_scale(eb));
+  return encode4(v[0].x, v[0].y, v[1].x, v[1].y, inv_scale(eb));
 }
 
 }  // namespace b8

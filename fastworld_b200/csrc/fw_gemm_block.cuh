@@ -54,22 +54,16 @@ __device__ __forceinline__ void umma_mx8_block(uint32_t one, uint32_t d, uint32_
     FW_MX8("1");
 #undef FW_MX8
 }
-// 32 rows of 16 bytes (512 contiguous bytes of shared memory) to four columns of Tensor Memory, the same
-// in every lane quarter: lane l of column c gets word c of row l.  Runs in order with the MMAs of the issuing lane.
-template <int CG>
-__device__ __forceinline__ void tmem_copy_if(uint32_t one, uint32_t taddr, uint32_t saddr) {
+// In both CTAs of a pair, 32 rows of 16 bytes (512 contiguous bytes of its shared memory) to four columns of its
+// Tensor Memory, the same in every lane quarter: lane l of column c gets word c of row l.  Runs in order with
+// the MMAs of the issuing lane.
+__device__ __forceinline__ void tmem_copy_pair_if(uint32_t one, uint32_t taddr, uint32_t saddr) {
   // descriptor: 128 bytes between 8-row groups, version 1, no swizzle
   const uint64_t desc = (uint64_t)((saddr >> 4) & 0x3fffu) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
-  if constexpr (CG == 2)
-    asm volatile(
-        "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %2, 0;\n\t"
-        "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(taddr), "l"(desc), "r"(one)
-        : "memory");
-  else
-    asm volatile(
-        "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %2, 0;\n\t"
-        "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(taddr), "l"(desc), "r"(one)
-        : "memory");
+  asm volatile(
+      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %2, 0;\n\t"
+      "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(taddr), "l"(desc), "r"(one)
+      : "memory");
 }
 
 // Low word of a tile's descriptor: address and (unused with this swizzle) leading offset.

@@ -59,7 +59,8 @@ __device__ __forceinline__ void write_row4(const BlockGemmArgs& a, int m, int n,
   const float2 x = activate2<ACT>(make_float2(u.x + bias[0], u.y + bias[1]));
   const float2 y = activate2<ACT>(make_float2(u.z + bias[2], u.w + bias[3]));
   if constexpr (OUT == FW_U8) {
-    const float v[4] = {n < N ? x.x : 0.f, n + 1 < N ? x.y : 0.f, n + 2 < N ? y.x : 0.f, n + 3 < N ? y.y : 0.f};
+    const float2 v[2] = {make_float2(n < N ? x.x : 0.f, n + 1 < N ? x.y : 0.f),
+                         make_float2(n + 2 < N ? y.x : 0.f, n + 3 < N ? y.y : 0.f)};
     uint32_t eb;
     const uint32_t code = b8::encode_block(v, eb);
     const int blk = n / b8::BLK;
@@ -157,28 +158,25 @@ __global__ void __launch_bounds__(nk::THREADS)
         if (used >> s & 1u) mbar_wait(full + s, last_par >> s & 1u, &no_abort, nullptr, DEV_TIMEOUT_DRAIN);
     }
   } else if (warp == 1) {
-    {
-      const uint32_t one = lane == 0;
-      constexpr uint32_t idesc = idesc_mx8(128, BN);
-      bool ok = true;
-      for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
-        const int s = i % C::STAGES, grp = kb / b8::GRP - kb0 / b8::GRP, buf = grp & 1;
-        if (i == 0 || kb % b8::GRP == 0)
-          ok = wait_on(sf_full + buf, (uint32_t)(grp >> 1) & 1u, abort_flag);
-        if (ok) ok = wait_on(full + s, (uint32_t)(i / C::STAGES) & 1u, abort_flag);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t desc = desc_lo(smem_u32(smem + s * C::STAGE));
-        const uint32_t sf = tmem + (uint32_t)(C::SF_COL + buf * 8);
-        umma_mx8_block<1>(one, tmem, desc, desc + (C::P_BYTES >> 4), with_scale_byte(idesc, (uint32_t)(kb % b8::GRP)), sf, sf + 4,
-                          i != 0);
-        umma_commit_if<1>(one, empty + s);
-        if (kb % b8::GRP == b8::GRP - 1) umma_commit_if<1>(one, sf_free + buf);
-      }
-      umma_commit_if<1>(one, done);
-      volatile int no_abort = 0;
-      mbar_wait(done, 0, &no_abort, nullptr, DEV_TIMEOUT_DRAIN);
+    const uint32_t one = lane == 0;
+    constexpr uint32_t idesc = idesc_mx8(128, BN);
+    bool ok = true;
+    for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
+      const int s = i % C::STAGES, grp = kb / b8::GRP - kb0 / b8::GRP, buf = grp & 1;
+      if (i == 0 || kb % b8::GRP == 0) ok = wait_on(sf_full + buf, (uint32_t)(grp >> 1) & 1u, abort_flag);
+      if (ok) ok = wait_on(full + s, (uint32_t)(i / C::STAGES) & 1u, abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t desc = desc_lo(smem_u32(smem + s * C::STAGE));
+      const uint32_t sf = tmem + (uint32_t)(C::SF_COL + buf * 8);
+      umma_mx8_block<1>(one, tmem, desc, desc + (C::P_BYTES >> 4), with_scale_byte(idesc, (uint32_t)(kb % b8::GRP)), sf,
+                        sf + 4, i != 0);
+      umma_commit_if<1>(one, empty + s);
+      if (kb % b8::GRP == b8::GRP - 1) umma_commit_if<1>(one, sf_free + buf);
     }
+    umma_commit_if<1>(one, done);
+    volatile int no_abort = 0;
+    mbar_wait(done, 0, &no_abort, nullptr, DEV_TIMEOUT_DRAIN);
   } else if (warp < 6) {
     const int q = warp & 3;   // lane quarter of Tensor Memory
     const uint32_t quarter = tmem + ((uint32_t)(q * 32) << 16);

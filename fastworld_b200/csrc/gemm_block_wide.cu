@@ -161,7 +161,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
-          for (int c = 0; c < 3; ++c) tmem_copy_if<2>(one, sf + 4 * c, sf_smem + slot * SF_BYTES + 512 * c);
+          for (int c = 0; c < 3; ++c) tmem_copy_pair_if(one, sf + 4 * c, sf_smem + slot * SF_BYTES + 512 * c);
           uint32_t id = idesc_mx8(BM, BN);
           // a tile's first MMA: tile it - 1's shared columns have been read, and all of tile it - 2
           if (!accumulate && it > 0) ok = wait_on(tfree, (it - 1) & 1u, abort_flag);
