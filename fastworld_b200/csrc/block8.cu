@@ -174,8 +174,13 @@ __device__ __forceinline__ void norm_row(float2 (&x)[NB][2], int kind, float eps
   }
 }
 
+// Warps that an SM has to hold, which sets the registers: 48 of them (about 40 registers) measured 15.7 us at 2640 x 1536,
+// 40 11.7, 32 11.5 (but 23.7 against 22.4 at 6032 rows), as many as the compiler's 67 registers allow 12.0; at
+// 4680 x 5120 30 warps 56.3 us, 20 (69 registers) 63.7, 40 97.
+constexpr int norm_warps(int NB) { return NB <= 3 ? 40 : NB == 4 ? 32 : 16; }
+
 template <typename Y, bool VEC, int W, int NB>
-__global__ void __launch_bounds__(W * 32) norm_gate_resid_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(W * 32, norm_warps(NB) / W) norm_gate_resid_kernel(const NormArgs a) {
   pdl_trigger();
   pdl_wait();
   __shared__ float slots[4 * W];
