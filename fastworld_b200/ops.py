@@ -5,8 +5,6 @@ or with the wrong dtype/layout raises.
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
@@ -282,9 +280,13 @@ def norm_gate_resid_(resid: torch.Tensor, y=None, post=None, post_w=None, post_b
     if out == "e4m3":
         h, s = _block_empty(M, D, resid.device)
     elif out == "bf16":
-        h = torch.empty(M, D, device=resid.device, dtype=torch.bfloat16)
-    a = _lib.FwNormArgs(resid.data_ptr(), ptr(y), _lib.DT_F32 if y is not None and y.dtype is f32 else _lib.DT_BF16,
-                        NORMS[post], NORMS[pre], ptr(post_w), ptr(post_b), ptr(pre_w), ptr(pre_b), ptr(gate), ptr(shift),
-                        ptr(scale), resid_scale, branch_scale, eps, M, D, min(rpf, 2**31 - 1), ptr(h), ptr(s))
-    _on(index, lib().fw_norm_gate_resid, "norm_gate_resid", ctypes.byref(a))
-    return (h, s) if out == "e4m3" else h
+        h = torch.empty(M, D, device=resid.device, dtype=b16)
+    args = _lib.NORM_ARGS.pack(
+        resid.data_ptr(), 0 if y is None else y.data_ptr(), _lib.DT_F32 if y is not None and y.dtype is f32 else _lib.DT_BF16,
+        NORMS[post], NORMS[pre], 0 if post_w is None else post_w.data_ptr(), 0 if post_b is None else post_b.data_ptr(),
+        0 if pre_w is None else pre_w.data_ptr(), 0 if pre_b is None else pre_b.data_ptr(),
+        0 if gate is None else gate.data_ptr(), 0 if shift is None else shift.data_ptr(),
+        0 if scale is None else scale.data_ptr(), resid_scale, branch_scale, eps, M, D, min(rpf, 2**31 - 1),
+        0 if h is None else h.data_ptr(), 0 if s is None else s.data_ptr())
+    _on(index, lib().fw_norm_gate_resid, "norm_gate_resid", args)
+    return h if s is None else (h, s)
