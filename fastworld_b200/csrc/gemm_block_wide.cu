@@ -36,9 +36,18 @@ constexpr int SMEM = BAR_OFF + 256;
 constexpr int THREADS = 384, EPI0 = 4;        // first epilogue warp
 constexpr uint32_t SHIFT = 224;              // first column of the odd tiles' accumulator
 constexpr uint32_t SF_COL = 480, SF_STRIDE = 16;
-constexpr int AHEAD = 2;                     // groups that the exponents are fetched ahead
+constexpr int AHEAD = 1;                     // groups that the exponents are fetched ahead
 static_assert(SMEM <= 232448, "shared memory of a CTA");
 }  // namespace wide
+
+// Arrive on an mbarrier of either CTA, given by its shared::cluster address, without a release at cluster
+// scope: that waits for all that the thread has in flight, 0.6-1 us at every tile change and every group of
+// scales (2640 x 8960 x 1536 with GELU to e4m3 40.3 -> 34.9 us without it).  No data crosses to the other CTA by these arrivals:
+// what they announce is that Tensor Memory reads are complete (tcgen05.wait::ld), or that this CTA's own shared
+// memory holds scales which this CTA's tensor core reads (fence.proxy.async before the arrival).
+__device__ __forceinline__ void mbar_arrive_either(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
 
 // Rows of C leave through a warp's 4 KB box: 32 rows of 128 bytes, 128-byte swizzle, one TMA store
 // (the tensor map clips rows and columns that do not exist).
@@ -231,7 +240,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
       for (int c = 0; c < 3; ++c) dst[32 * c + lane] = make_uint4(w[0][4 * c], w[0][4 * c + 1], w[0][4 * c + 2], w[0][4 * c + 3]);
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(sf_full0 + 8u * slot);
+      if (lane == 0) mbar_arrive_either(sf_full0 + 8u * slot);
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i)
 #pragma unroll
@@ -291,7 +300,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
         tmem_ld_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(tfree0);
+        if (lane == 0) mbar_arrive_either(tfree0);
         scan(keep, first * 32);
 #pragma unroll 1
         for (int j = 1; j < 4; ++j) {
@@ -358,7 +367,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
         tmem_ld_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(tfree0);
+        if (lane == 0) mbar_arrive_either(tfree0);
 #pragma unroll 1
         for (int j = 0; j < 4; ++j) {
           const int c = first + dir * j;
