@@ -26,6 +26,10 @@ namespace {
 // Few tiles would leave most SMs idle and stream the weights through few of them, so the k-blocks of a tile are
 // split over a cluster of CTAs.  Each stages its partial accumulator in its own shared memory; then each takes
 // every splits-th row, adds the partials of all ranks in rank order (the same sum on every run) and writes it.
+//
+// What bounds it: with a few rows the weights' bytes behind about 4 us of launch, first loads and result
+// (1 x 1536 x 1536 4.8 us; 1 x 5120 x 13824, 71 MB, 15.4 us or 4.6 TB/s); with a few hundred rows the chain of
+// k-blocks of a CTA, 0.5 us each, which the split shortens for a join of 2.7 us (of 12.3 us at 512 x 1536 x 4096).
 namespace nk {
 constexpr int THREADS = 192, MAX_SPLITS = 8;
 template <int BN>
@@ -327,15 +331,22 @@ int launch_nk(const void* A8, const void* B8, const BlockGemmArgs& a, cudaStream
   }
 }
 
-// Which kernel, tile and split: the least of a time model (us) whose constants were fitted to 70 measured
-// sizes (1 to 4000 rows, 30 to 13824 columns, 60 to 8960 of K): its choice is 2 % off the best variant on average,
-// 30 % at worst.  Small tiles: launch, then the busiest SM's operand bytes, or the latency of a CTA's chain
-// of k-blocks, or HBM, then the exposed epilogue and the join of a split; wide kernel: waves of 256 x 256 tiles.
-// Both sides, measured: 880 x 1536 x 8960 18.4 us on 128-row tiles split 3 ways, 31.2 us wide; 2640 x 1536 x 1536
-// 14.1 and 11.0 us; 512 x 1536 x 4096 12.2 us split 5 ways, 16.0 us unsplit, 17.9 us wide; 1 x 9216 x 1536 6.9 us
-// split 4 ways, 6.7 us unsplit; 1 x 1536 x 1536 4.7 us split 6 ways, 6.3 us unsplit.  A split's CTAs fill at most
-// 9/10 of two per SM: clusters do not fit every SM of a GPC, and what is left over waits for whole tiles to end
-// (512 x 1536 x 4096 on 64-row tiles split 3 ways, 288 CTAs: 18.6 us).
+// Which kernel, tile and split: the least of a time model (us) whose constants were fitted to measured times
+// (small tiles: 70 sizes of 1 to 4000 rows, 30 to 13824 columns, 60 to 8960 of K; between the two kernels: 34 sizes,
+// where its choice is the faster one but for four, 1, 6, 8 and 24 % off).  Small tiles: launch, then the busiest
+// SM's operand bytes, or the latency of a CTA's chain of k-blocks, or HBM, then the exposed epilogue and the
+// join of a split; wide kernel: waves of 256 x 256 tiles, more for rows that no TMA store can address.
+// Both sides, measured (us):
+//   small tiles   880 x 1536 x 8960   20.4 (split 3 ways; 30.9 unsplit)   26.6 wide
+//                 512 x 1536 x 13824  19.2                                38.1 wide
+//                 1001 x 777 x 1283    7.5                                10.7 wide
+//                 512 x 1536 x 4096   12.3 (split 5 ways; 16.2 unsplit)   17.9 wide
+//   wide         2640 x 1536 x 1536   10.0 small tiles                     9.5 wide
+//                 512 x 13824 x 5120  45.4                                34.7
+//                6032 x 1536 x 1536   19.7                                14.5
+//   a split         1 x 1536 x 1536    4.8 split 6 ways, 6.2 unsplit; 1 x 9216 x 1536 7.0 split 4 ways, 6.8 unsplit
+// A split's CTAs fill at most 9/10 of two per SM: clusters do not fit every SM of a GPC, and what is left over
+// waits for whole tiles to end (512 x 1536 x 4096 on 64-row tiles split 3 ways, 288 CTAs: 18.6 us).
 struct Plan {
   int bn, splits;   // bn 0: the wide kernel
 };
@@ -346,7 +357,7 @@ Plan make_plan(int M, int N, int num_kb, int out_dtype) {
   const long long waves = up(up(M, 256) * up(N, 256), sms / 2);
   const bool tma_out = out_dtype == FW_U8 || N % (out_dtype == FW_F32 ? 4 : 8) == 0;
   Plan best = {0, 1};
-  double least = 5.7 + waves * (num_kb * 0.3 + (tma_out ? 1.0 : 3.5));
+  double least = 4.0 + waves * (num_kb * 0.37 + (tma_out ? 0.4 : 1.9));
   for (int bn = 16; bn <= 128; bn *= 2) {
     if (up(M, bn) > 65535) continue;
     const long long tiles = up(N, 128) * up(M, bn);

@@ -16,7 +16,12 @@
 // Every wait is bounded; a wait that runs out makes both CTAs unwind.
 //
 // What bounds it: the MMAs alone take 0.30 us per k-block of 256 x 256 x 128 (their operands leave shared memory
-// while the next ones enter it), with loads and scales 0.36-0.38 us; a tile change costs about 1 us.
+// while the next ones enter it), with loads and scales 0.37 us; a call adds 4 us (first tile, last epilogue) and
+// a tile change 0.4 us.  2640 rows, bf16 result: 4608 x 1536 18.5 us (2.0 PFLOP/s), 8960 x 1536 33.2 (2.2), 1536 x 8960
+// 30.3 (2.4); 4680 x 13824 x 5120 237 us (2.8), and 290 us when it repeats for seconds at the power limit.
+// Tried: tiles of 240 columns whose accumulators do not overlap (18.5 -> 20.7 us, 237 -> 260), four stages (240 ->
+// 245), a store wait and an exit barrier without release (18.5 -> 18.2; but then arrivals at a CTA that has left
+// are excluded by timing only).
 #include "fw_gemm_block.cuh"
 
 namespace fw {
@@ -36,15 +41,15 @@ constexpr int SMEM = BAR_OFF + 256;
 constexpr int THREADS = 384, EPI0 = 4;        // first epilogue warp
 constexpr uint32_t SHIFT = 224;              // first column of the odd tiles' accumulator
 constexpr uint32_t SF_COL = 480, SF_STRIDE = 16;
-constexpr int AHEAD = 1;                     // groups that the exponents are fetched ahead
 static_assert(SMEM <= 232448, "shared memory of a CTA");
 }  // namespace wide
 
-// Arrive on an mbarrier of either CTA, given by its shared::cluster address, without a release at cluster
-// scope: that waits for all that the thread has in flight, 0.6-1 us at every tile change and every group of
-// scales (2640 x 8960 x 1536 with GELU to e4m3 40.3 -> 34.9 us without it).  No data crosses to the other CTA by these arrivals:
-// what they announce is that Tensor Memory reads are complete (tcgen05.wait::ld), or that this CTA's own shared
-// memory holds scales which this CTA's tensor core reads (fence.proxy.async before the arrival).
+// Arrive on an mbarrier of either CTA, given by its shared::cluster address, without a release at cluster scope:
+// that waits for all that the thread has in flight, 0.6-1 us at every tile change and every group of scales
+// (2640 x 8960 x 1536 with GELU to e4m3 40.3 -> 34.9 us without it).  No thread of the other CTA reads what was
+// written before these arrivals.  They announce that Tensor Memory reads are complete (tcgen05.wait::ld), or that
+// this CTA's own shared memory holds scales, which its own tensor core reads: every lane's fence.proxy.async,
+// which completes the lane's writes towards that reader, comes before the arrival.
 __device__ __forceinline__ void mbar_arrive_either(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
@@ -209,9 +214,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
     }
   } else if (warp == 2) {
     const uint32_t sf_full0 = mapa_cluster(sf_full, 0);
-    // Words are fetched AHEAD groups before they are stored: the loads queue behind the tiles' traffic, and
-    // one group's MMAs do not cover their latency.
-    uint32_t w[AHEAD + 1][12];
+    // A group is fetched before the last one is stored: the loads queue behind the tiles' traffic (fetched two
+    // groups ahead, 2640 x 4608 x 1536 takes 18.9 us instead of 18.6).
+    uint32_t w[12], next[12];
     int lt = pair, lg = 0;   // next group to fetch
     auto fetch = [&](uint32_t(&v)[12]) {
       if (lt < num_tiles) {
@@ -228,23 +233,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
         }
       }
     };
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) fetch(w[i]);
+    fetch(w);
     const uint32_t groups = pair < num_tiles ? (uint32_t)((num_tiles - 1 - pair) / npairs + 1) * (uint32_t)num_g : 0;
     for (uint32_t grp = 0; grp < groups; ++grp) {
-      fetch(w[AHEAD]);
+      fetch(next);
       const uint32_t slot = grp % SF_RING;
       if (!__all_sync(0xffffffffu, wait_on(sf_free + slot, ((grp / SF_RING) & 1u) ^ 1u, abort_flag))) break;
       uint4* dst = reinterpret_cast<uint4*>(smem + SF_OFF + slot * SF_BYTES);
 #pragma unroll
-      for (int c = 0; c < 3; ++c) dst[32 * c + lane] = make_uint4(w[0][4 * c], w[0][4 * c + 1], w[0][4 * c + 2], w[0][4 * c + 3]);
+      for (int c = 0; c < 3; ++c) dst[32 * c + lane] = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive_either(sf_full0 + 8u * slot);
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i)
-#pragma unroll
-        for (int c = 0; c < 12; ++c) w[i][c] = w[i + 1][c];
+      for (int c = 0; c < 12; ++c) w[c] = next[c];
     }
   } else if (warp >= EPI0) {
     const int q = warp & 3, h = (warp - EPI0) >> 2;
