@@ -59,7 +59,7 @@ struct Four<__half, true> {
 // A warp takes one row's group of 512 columns: four blocks, four columns per lane and block, so
 // each load and each store of codes is contiguous over the warp and a block's maximum is one warp
 // reduction.  The eight warps of a CTA take eight neighbouring rows, whose words of exponents are one 32-byte
-// sector.  Many short CTAs keep HBM busiest: 2640 x 8960 bf16 in 13.2 us (5.4 TB/s); warps that took two,
+// sector.  Many short CTAs keep HBM busiest: 2640 x 8960 bf16 in 12.9 us (5.5 TB/s); warps that took two,
 // three or six groups with the next one's loads in flight took 16.0, 16.2 and 17.3 us.
 constexpr int QROWS = 8;
 
@@ -117,10 +117,11 @@ struct NormArgs {
 
 // One row per CTA of W warps; warp w holds blocks [w NB, w NB + NB) of 128 columns in
 // registers, four columns per lane and block.  HBM bounds it (12 bytes per element in bf16), but a row's bytes wait
-// behind up to four sums over the row, so many rows have to be in flight: 2640 x 1536 in 11.0 us (4.4 TB/s),
-// 6032 x 1536 in 20.9 us (5.3 TB/s), 4680 x 5120 in 66.8 us (4.3 TB/s).  Slower: CTAs that take several rows,
+// behind up to four sums over the row, so many rows have to be in flight: 2640 x 1536 in 11.7 us (4.2 TB/s),
+// 6032 x 1536 in 22.4 us (5.0 TB/s), 4680 x 5120 in 56.4 us (5.1 TB/s).  Slower: CTAs that take several rows,
 // the next one's loads in flight (16.8 us at 2640 x 1536), and rows brought to a ring in shared memory by bulk copies
-// with a warp or four per row (27 us): fewer warps per SM are left to work through the sums.
+// with a warp or four per row (27 us): fewer warps per SM are left to work through the sums; and mean and square in
+// one sum of three numbers, joined pairwise (13.4 us).
 template <int W>
 __device__ __forceinline__ float row_sum(float v, float* slot, int warp, int lane) {
 #pragma unroll
@@ -174,9 +175,9 @@ __device__ __forceinline__ void norm_row(float2 (&x)[NB][2], int kind, float eps
   }
 }
 
-// Warps that an SM has to hold, which sets the registers: 48 of them (about 40 registers) measured 15.7 us at 2640 x 1536,
-// 40 11.7, 32 11.5 (but 23.7 against 22.4 at 6032 rows), as many as the compiler's 67 registers allow 12.0; at
-// 4680 x 5120 30 warps 56.3 us, 20 (69 registers) 63.7, 40 97.
+// Warps that an SM has to hold, which sets the registers: 48 of them (about 40 registers) measured 15.7 us at
+// 2640 x 1536, 40 11.7, 32 11.5 (but 23.7 against 22.4 at 6032 rows), as many as the compiler's 67 registers allow
+// 12.0; at 4680 x 5120 30 warps 56.3 us, 20 (69 registers) 63.7, 40 97.
 constexpr int norm_warps(int NB) { return NB <= 3 ? 40 : NB == 4 ? 32 : 16; }
 
 template <typename Y, bool VEC, int W, int NB>
@@ -305,8 +306,9 @@ __global__ void __launch_bounds__(W * 32, norm_warps(NB) / W) norm_gate_resid_ke
       a.out_s[((size_t)(blk / b8::GRP) * a.M + row) * b8::GRP + blk % b8::GRP] = 127;
 }
 
-// Warps per row and blocks per warp by the row's width: at 1536 columns 4 x 3 measured 11.1 us for 2640 rows, 6 x 2
-// 12.2, 12 x 1 16.1 and 2 x 6 12.1; at 5120 columns 10 x 4 66.8 us for 4680 rows, 14 x 3 65.9, 8 x 6 68.4, 20 x 2 105.
+// Warps per row and blocks per warp by the row's width, each at the registers that the compiler gave it: at 1536
+// columns 4 x 3 measured 11.1 us for 2640 rows, 6 x 2 12.2, 12 x 1 16.1 and 2 x 6 12.1; at 5120 columns 10 x 4
+// 66.8 us for 4680 rows, 14 x 3 65.9, 8 x 6 68.4, 20 x 2 105.
 template <typename Y, bool VEC>
 int norm_launch(const NormArgs& a, cudaStream_t s) {
   const int nb = b8::blocks(a.D);

@@ -84,7 +84,9 @@ __device__ __forceinline__ uint32_t encode4_finite(float a, float b, float c, fl
 }
 // Four codes of x * inv (round to nearest even; NaN and infinities become the NaN code).
 __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, float inv) {
-  auto in = [&](float v) { return (__float_as_uint(v) & 0x7fffffffu) < 0x7f800000u ? v * inv : __uint_as_float(0x7fffffffu); };
+  auto in = [&](float v) {
+    return (__float_as_uint(v) & 0x7fffffffu) < 0x7f800000u ? v * inv : __uint_as_float(0x7fffffffu);
+  };
   uint16_t lo, hi;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(in(b)), "f"(in(a)));
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(in(d)), "f"(in(c)));

@@ -23,7 +23,9 @@ __host__ __device__ constexpr uint32_t idesc_mx8(int M, int N) {
   return ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((uint32_t)(M >> 4) << 24);
 }
 // ... with byte `id` of the scale words of both operands
-__device__ __forceinline__ uint32_t with_scale_byte(uint32_t idesc, uint32_t id) { return idesc | (id << 4) | (id << 29); }
+__device__ __forceinline__ uint32_t with_scale_byte(uint32_t idesc, uint32_t id) {
+  return idesc | (id << 4) | (id << 29);
+}
 
 // The four MMAs of a k-block (128 of K, 32 each), issued by the lane with `one` != 0 while the whole warp
 // runs the loop around them: control flow and operands then stay uniform, where a branch on the lane

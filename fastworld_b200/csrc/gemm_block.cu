@@ -57,8 +57,8 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {   // shared memor
 
 // v: columns [n, n + 4) of row m of C before the bias; columns that do not exist hold anything.
 template <int ACT, int OUT>
-__device__ __forceinline__ void write_row4(const BlockGemmArgs& a, int m, int n, const float4& u, const float (&bias)[4],
-                                           bool vec) {
+__device__ __forceinline__ void write_row4(const BlockGemmArgs& a, int m, int n, const float4& u,
+                                           const float (&bias)[4], bool vec) {
   const int N = a.N;
   const float2 x = activate2<ACT>(make_float2(u.x + bias[0], u.y + bias[1]));
   const float2 y = activate2<ACT>(make_float2(u.z + bias[2], u.w + bias[3]));
@@ -311,7 +311,8 @@ int launch_nk(const void* A8, const void* B8, const BlockGemmArgs& a, cudaStream
     ++cfg.numAttrs;
   }
   auto go = [&](auto kern) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return FW_ECUDA;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
+      return FW_ECUDA;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tp, tq, a);
     note_launch();
     return e == cudaSuccess ? FW_OK : FW_ECUDA;

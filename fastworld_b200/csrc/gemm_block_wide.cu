@@ -78,9 +78,10 @@ __device__ __forceinline__ void finish(float2 (&v)[16], const uint32_t (&r)[32],
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float4 b = *reinterpret_cast<const float4*>(bias + 4 * i);
-    v[2 * i] = activate2<ACT>(__fadd2_rn(make_float2(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1])), make_float2(b.x, b.y)));
-    v[2 * i + 1] =
-        activate2<ACT>(__fadd2_rn(make_float2(__uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3])), make_float2(b.z, b.w)));
+    const float2 x = make_float2(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]));
+    const float2 y = make_float2(__uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3]));
+    v[2 * i] = activate2<ACT>(__fadd2_rn(x, make_float2(b.x, b.y)));
+    v[2 * i + 1] = activate2<ACT>(__fadd2_rn(y, make_float2(b.z, b.w)));
   }
 }
 
@@ -337,7 +338,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               const uint32_t* y = x + 16 * h16 + 4 * k;
-              const float e0 = __uint_as_float(y[0]), e1 = __uint_as_float(y[1]), e2 = __uint_as_float(y[2]), e3 = __uint_as_float(y[3]);
+              const float e0 = __uint_as_float(y[0]), e1 = __uint_as_float(y[1]);
+              const float e2 = __uint_as_float(y[2]), e3 = __uint_as_float(y[3]);
               w[k] = finite ? b8::encode4_finite(e0, e1, e2, e3, inv) : b8::encode4(e0, e1, e2, e3, inv);
             }
             box_put(box, lane, 2 * c + h16, make_uint4(w[0], w[1], w[2], w[3]));
@@ -469,10 +471,11 @@ int gemm_block_wide_launch(const void* A8, const void* B8, const BlockGemmArgs& 
   };
   using Yes = std::integral_constant<bool, true>;
   using No = std::integral_constant<bool, false>;
+  const std::integral_constant<int, FW_F32> f32;
+  const std::integral_constant<int, FW_BF16> b16;
   if (a.out_dtype == FW_U8) return by_act(std::integral_constant<int, FW_U8>{}, Yes{});
-  if (a.out_dtype == FW_F32)
-    return tma_out ? by_act(std::integral_constant<int, FW_F32>{}, Yes{}) : by_act(std::integral_constant<int, FW_F32>{}, No{});
-  return tma_out ? by_act(std::integral_constant<int, FW_BF16>{}, Yes{}) : by_act(std::integral_constant<int, FW_BF16>{}, No{});
+  if (a.out_dtype == FW_F32) return tma_out ? by_act(f32, Yes{}) : by_act(f32, No{});
+  return tma_out ? by_act(b16, Yes{}) : by_act(b16, No{});
 }
 
 }  // namespace fw
