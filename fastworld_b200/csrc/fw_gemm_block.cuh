@@ -89,6 +89,14 @@ __device__ __forceinline__ void umma_commit_if(uint32_t one, uint64_t* bar) {
         : "memory");
 }
 
+// ... a pair's MMAs, on this CTA's barrier alone.
+__device__ __forceinline__ void umma_commit_local_if(uint32_t one, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)), "r"(one)
+      : "memory");
+}
+
 // One 32-bit column per register, this warp's lane quarter.
 template <int N>
 __device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[N]);

@@ -4,10 +4,10 @@
 // the 48 KB of a 128 x 256 tile on one CTA), and each one's Tensor Memory gets its 128 rows of the
 // accumulator, all 256 columns.  Persistent over tiles; 12 warps per CTA:
 //   warp 0      TMA producer of this CTA's halves (loads complete on the even CTA's `full`);
-//   warp 1      even CTA: the one MMA issuer of the pair, which also copies the scales to Tensor Memory (tcgen05.cp,
-//               in order with the MMAs); both: Tensor Memory of the pair;
+//   warp 1      even CTA: the one MMA issuer of the pair; both: Tensor Memory of the pair;
 //   warp 2      exponent words of A's 128 rows and of all 256 rows of B to this CTA's shared memory, a group of
 //               512 of K at a time, in the order that the copy reads;
+//   warp 3      even CTA: copies them to the Tensor Memory of both (tcgen05.cp), two buffers of a group each;
 //   warps 4-11  epilogue: lane quarter w % 4, column half (w - 4) / 4.
 // Tensor Memory has 512 columns; two accumulators of 256 and the 24 of the scales do not
 // fit side by side, so the accumulators overlap by 32 columns: even tiles at [0, 256), odd ones at [224, 480),
@@ -94,18 +94,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + BAR_OFF);
   uint64_t* empty = full + STAGES;
-  uint64_t* sf_full = empty + STAGES;    // [SF_RING], even CTA's
-  uint64_t* sf_free = sf_full + SF_RING;
+  uint64_t* sf_full = empty + STAGES;    // [SF_RING] a group's exponents are in both CTAs' shared memory, even CTA's
+  uint64_t* sf_free = sf_full + SF_RING; // [SF_RING] ... are copied to Tensor Memory
   uint64_t* tfull = sf_free + SF_RING;   // [2] accumulator of an even / odd tile complete
   uint64_t* tfree = tfull + 2;           // [1] the shared columns of the last tile are read, even CTA's
-  uint64_t* drain = tfree + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint64_t* sf_used = tfree + 1;         // [2] MMAs have read a buffer of scales in Tensor Memory, even CTA's
+  uint64_t* drain = sf_used + 2;         // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
   const int num_m = (a.M + BM - 1) / BM, num_n = (a.N + BN - 1) / BN, num_tiles = num_m * num_n;
   const int num_kb = a.K / b8::BLK, num_g = (num_kb + b8::GRP - 1) / b8::GRP;
+  const uint32_t groups = pair < num_tiles ? (uint32_t)((num_tiles - 1 - pair) / npairs + 1) * (uint32_t)num_g : 0;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -116,9 +118,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
       mbar_init(sf_free + b, 1);
       mbar_init(sf_full + b, 2);   // one arrival per warp: those of all lanes queue up on the barrier
     }
-    for (int b = 0; b < 2; ++b) mbar_init(tfull + b, 1);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(tfull + b, 1);
+      mbar_init(sf_used + b, 1);
+      mbar_init(drain + b, 1);
+    }
     mbar_init(tfree, 2 * EPI_WARPS);
-    mbar_init(drain, 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -165,18 +170,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
       // computed in it.
       constexpr uint32_t SCALE_BYTE = (1u << 4) | (1u << 29);   // next byte of both operands' scale words
       const uint32_t desc0 = desc_lo(smem_u32(smem));
-      uint32_t stage = 0, phase = 0, desc = desc0, slot = 0, slot_phase = 0, sf = tmem + SF_COL, it = 0;
-      const uint32_t sf_smem = smem_u32(smem + SF_OFF);
+      uint32_t stage = 0, phase = 0, desc = desc0, slot = 0, slot_phase = 0, buf = 0, it = 0;
       bool ok = true;
       for (int t = pair; t < num_tiles && ok; t += npairs, ++it) {
         const uint32_t d = tmem + (it & 1u) * SHIFT;
         uint32_t accumulate = 0;
         for (int left = num_kb; left > 0;) {
-          ok = wait_on(sf_full + slot, slot_phase, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
-#pragma unroll
-          for (int c = 0; c < 3; ++c) tmem_copy_pair_if(one, sf + 4 * c, sf_smem + slot * SF_BYTES + 512 * c);
+          ok = wait_on(sf_free + slot, slot_phase, abort_flag);   // copied
+          const uint32_t sf = tmem + SF_COL + buf * SF_STRIDE;
           uint32_t id = idesc_mx8(BM, BN);
           // a tile's first MMA: tile it - 1's shared columns have been read, and all of tile it - 2
           if (!accumulate && it > 0) ok = wait_on(tfree, (it - 1) & 1u, abort_flag);
@@ -198,9 +199,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
             }
           }
           if (!ok) break;
-          umma_commit_if<2>(one, sf_free + slot);
+          umma_commit_local_if(one, sf_used + buf);
           left -= n;
-          sf ^= SF_STRIDE;   // the other of two buffers
+          buf ^= 1u;
           if (++slot == SF_RING) {
             slot = 0;
             slot_phase ^= 1u;
@@ -212,6 +213,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
       if (one) umma_commit_pair(smem_u32(drain));   // this CTA's only: nothing arrives at a CTA that has left
       volatile int no_abort = 0;
       mbar_wait(drain, 0, &no_abort, nullptr, DEV_TIMEOUT_DRAIN);
+    }
+  } else if (warp == 3) {
+    if (rank == 0) {
+      // not by the MMA issuer: the three copies cost it 0.2 us per group (4680 x 7680 x 5120 134 us, 130 this way)
+      const uint32_t one = lane == 0;
+      const uint32_t sf_smem = smem_u32(smem + SF_OFF);
+      for (uint32_t grp = 0; grp < groups; ++grp) {
+        const uint32_t slot = grp % SF_RING, buf = grp & 1u;
+        if (!wait_on(sf_full + slot, (grp / SF_RING) & 1u, abort_flag)) break;
+        if (!wait_on(sf_used + buf, ((grp >> 1) & 1u) ^ 1u, abort_flag)) break;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < 3; ++c)
+          tmem_copy_pair_if(one, tmem + SF_COL + buf * SF_STRIDE + 4 * c, sf_smem + slot * SF_BYTES + 512 * c);
+        umma_commit_if<2>(one, sf_free + slot);
+      }
+      if (one) umma_commit_pair(smem_u32(drain + 1));
+      volatile int no_abort = 0;
+      mbar_wait(drain + 1, 0, &no_abort, nullptr, DEV_TIMEOUT_DRAIN);
     }
   } else if (warp == 2) {
     const uint32_t sf_full0 = mapa_cluster(sf_full, 0);
@@ -235,7 +255,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
       }
     };
     fetch(w);
-    const uint32_t groups = pair < num_tiles ? (uint32_t)((num_tiles - 1 - pair) / npairs + 1) * (uint32_t)num_g : 0;
     for (uint32_t grp = 0; grp < groups; ++grp) {
       fetch(next);
       const uint32_t slot = grp % SF_RING;
