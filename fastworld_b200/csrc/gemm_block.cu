@@ -333,18 +333,18 @@ int launch_nk(const void* A8, const void* B8, const BlockGemmArgs& a, cudaStream
 }
 
 // Which kernel, tile and split: the least of a time model (us) whose constants were fitted to measured times
-// (small tiles: 70 sizes of 1 to 4000 rows, 30 to 13824 columns, 60 to 8960 of K; between the two kernels: 34 sizes,
-// where its choice is the faster one but for four, 1, 6, 8 and 24 % off).  Small tiles: launch, then the busiest
-// SM's operand bytes, or the latency of a CTA's chain of k-blocks, or HBM, then the exposed epilogue and the
-// join of a split; wide kernel: waves of 256 x 256 tiles, more for rows that no TMA store can address.
+// (small tiles: 70 sizes of 1 to 4000 rows, 30 to 13824 columns, 60 to 8960 of K; between the two kernels: 37 sizes, where
+// its choice is the faster one but for two, 4 and 7 % off).  Small tiles: launch, then the busiest SM's operand
+// bytes, or the latency of a CTA's chain of k-blocks, or HBM, then the exposed epilogue and the join of a split; wide
+// kernel: waves of 256 x 256 tiles, more for rows that no TMA store can address.
 // Both sides, measured (us):
-//   small tiles   880 x 1536 x 8960   20.4 (split 3 ways; 30.9 unsplit)   26.6 wide
-//                 512 x 1536 x 13824  19.2                                38.1 wide
+//   small tiles   880 x 1536 x 8960   20.4 (split 3 ways; 30.9 unsplit)   25.5 wide
+//                 512 x 1536 x 13824  19.1                                36.5 wide
 //                 1001 x 777 x 1283    7.5                                10.7 wide
 //                 512 x 1536 x 4096   12.3 (split 5 ways; 16.2 unsplit)   17.9 wide
-//   wide         2640 x 1536 x 1536   10.0 small tiles                     9.5 wide
-//                 512 x 13824 x 5120  45.4                                34.7
-//                6032 x 1536 x 1536   19.7                                14.5
+//   wide         2640 x 1536 x 1536   9.9 small tiles                     9.5 wide
+//                 512 x 13824 x 5120  44.6                                33.9
+//                6032 x 1536 x 1536   19.7                                14.4
 //   a split         1 x 1536 x 1536    4.8 split 6 ways, 6.2 unsplit; 1 x 9216 x 1536 7.0 split 4 ways, 6.8 unsplit
 // A split's CTAs fill at most 9/10 of two per SM: clusters do not fit every SM of a GPC, and what is left over
 // waits for whole tiles to end (512 x 1536 x 4096 on 64-row tiles split 3 ways, 288 CTAs: 18.6 us).
@@ -355,10 +355,11 @@ Plan make_plan(int M, int N, int num_kb, int out_dtype) {
   const int sms = num_sms();
   auto up = [](long long x, long long y) { return (x + y - 1) / y; };
   const double hbm = (((double)M + N) * num_kb * b8::BLK + 2.0 * M * N) / 5.2e6;
-  const long long waves = up(up(M, 256) * up(N, 256), sms / 2);
+  const long long wide = up(M, 256) * up(N, 256), waves = up(wide, sms / 2);
   const bool tma_out = out_dtype == FW_U8 || N % (out_dtype == FW_F32 ? 4 : 8) == 0;
   Plan best = {0, 1};
-  double least = 4.0 + waves * (num_kb * 0.37 + (tma_out ? 0.4 : 1.9));
+  const double kb_us = 0.27 + 0.08 * fmin(1.0, wide / (sms * 0.5));   // of a k-block, on one pair and on all
+  double least = 4.9 + waves * (num_kb * kb_us + (tma_out ? 0.4 : 1.9));
   for (int bn = 16; bn <= 128; bn *= 2) {
     if (up(M, bn) > 65535) continue;
     const long long tiles = up(N, 128) * up(M, bn);
@@ -367,7 +368,7 @@ Plan make_plan(int M, int N, int num_kb, int out_dtype) {
       const double per_sm = (double)up(tiles * sp, sms), kbs = (double)up(num_kb, sp);
       const double load = per_sm * kbs * (128 + bn) * b8::BLK / 1.8e5;
       const double chain = up(tiles * sp, 2 * sms) * kbs * 0.5;
-      const double t = 1.7 + fmax(fmax(load, chain), hbm) + 0.9 * bn / 128 * per_sm + (sp > 1 ? 3.4 : 0.0);
+      const double t = 1.7 + fmax(fmax(load, chain), hbm) + 0.9 * bn / 128 * per_sm + (sp == 1 ? 0.0 : bn == 128 ? 4.6 : 3.4);
       if (t < least) {
         least = t;
         best = {bn, sp};

@@ -15,13 +15,15 @@
 // odd tile's first) and the next tile's MMAs start once it has, so they still run under the rest of the epilogue.
 // Every wait is bounded; a wait that runs out makes both CTAs unwind.
 //
-// What bounds it: the MMAs alone take 0.30 us per k-block of 256 x 256 x 128 (their operands leave shared memory
-// while the next ones enter it), with loads and scales 0.37 us; a call adds 4 us (first tile, last epilogue) and
-// a tile change 0.4 us.  2640 rows, bf16 result: 4608 x 1536 18.5 us (2.0 PFLOP/s), 8960 x 1536 33.2 (2.2), 1536 x 8960
-// 30.3 (2.4); 4680 x 13824 x 5120 237 us (2.8), and 290 us when it repeats for seconds at the power limit.
+// What bounds it: the tensor core needs 2048 cycles for four k-blocks of 256 x 256 x 128, and their issue takes
+// 2240 (270 cycles for a block's four MMAs, 100 for its wait, 60 for its commit), 0.30 us a block; with all pairs' loads
+// 0.36 us.  A call adds 4 us (first tile, last epilogue), a tile change 0.4 us.  2640 rows, bf16 result: 4608 x 1536 18.2 us
+// (2.05 PFLOP/s), 8960 x 1536 32.6 (2.2), 1536 x 8960 29.3 (2.5); 4680 x 13824 x 5120 233 us (2.8), and 271 us when it
+// repeats for seconds at the power limit.
 // Tried: tiles of 240 columns whose accumulators do not overlap (18.5 -> 20.7 us, 237 -> 260), four stages (240 ->
 // 245), a store wait and an exit barrier without release (18.5 -> 18.2; but then arrivals at a CTA that has left
-// are excluded by timing only).
+// are excluded by timing only); halves of 128 columns for a last wave that leaves pairs idle (issue takes as long
+// for a half: 880 x 1536 x 8960 26.6 -> 27.4); the next wait tried before a block's MMAs (30.1 -> 31.0).
 #include "fw_gemm_block.cuh"
 
 namespace fw {
