@@ -257,10 +257,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
       }
     };
     fetch(w);
+    bool ok = true;
     for (uint32_t grp = 0; grp < groups; ++grp) {
       fetch(next);
       const uint32_t slot = grp % SF_RING;
-      if (!__all_sync(0xffffffffu, wait_on(sf_free + slot, ((grp / SF_RING) & 1u) ^ 1u, abort_flag))) break;
+      ok = __all_sync(0xffffffffu, wait_on(sf_free + slot, ((grp / SF_RING) & 1u) ^ 1u, abort_flag));
+      if (!ok) break;
       uint4* dst = reinterpret_cast<uint4*>(smem + SF_OFF + slot * SF_BYTES);
 #pragma unroll
       for (int c = 0; c < 3; ++c) dst[32 * c + lane] = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
@@ -270,6 +272,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
 #pragma unroll
       for (int c = 0; c < 12; ++c) w[c] = next[c];
     }
+    // the last copies' arrivals from the even CTA have come: none is under way to this CTA at exit
+    for (uint32_t grp = groups < SF_RING ? 0 : groups - SF_RING; grp < groups && ok; ++grp)
+      ok = wait_on(sf_free + grp % SF_RING, (grp / SF_RING) & 1u, abort_flag);
   } else if (warp >= EPI0) {
     const int q = warp & 3, h = (warp - EPI0) >> 2;
     const uint32_t tfree0 = mapa_cluster(tfree, 0);

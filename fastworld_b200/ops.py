@@ -237,7 +237,8 @@ def norm_gate_resid_(resid: torch.Tensor, y=None, post=None, post_w=None, post_b
     resid fp32 [M, D]; y bf16 or fp32 [M, D], or None (no residual update); post and pre 'layer', 'rms' or None,
     fp32 statistics; weights bf16 [D]; gate, shift and scale fp32 [frames, D] (or [D], one frame) with
     f = row // rows_per_frame (None: all rows are one frame).  out: 'bf16', 'e4m3' (the pair (q, s) of
-    quant_e4m3_block, quantised from fp32) or None (h is not computed)."""
+    quant_e4m3_block, quantised from fp32) or None (h is not computed).  resid's memory may be y's as a whole
+    (fp32), and otherwise overlaps no argument."""
     f32, b16, index, shape = torch.float32, torch.bfloat16, resid.get_device(), resid.shape
     if index < 0 or len(shape) != 2 or shape[1] == 0 or resid.dtype is not f32 or not resid.is_contiguous():
         _refuse("resid", resid, f32, index, "[M, D > 0]")
@@ -257,7 +258,8 @@ def norm_gate_resid_(resid: torch.Tensor, y=None, post=None, post_w=None, post_b
                 and branch_scale == 1.0):
             raise ValueError("post, post_w, post_b, gate, resid_scale and branch_scale need y")
     else:
-        if (y.dtype is not b16 and y.dtype is not f32) or y.shape != shape or y.get_device() != index or not y.is_contiguous():
+        if ((y.dtype is not b16 and y.dtype is not f32) or y.shape != shape or y.get_device() != index
+                or not y.is_contiguous()):
             _refuse("y", y, "bf16 or fp32", index, [M, D])
         if post_w is not None:
             _weight("post_w", post_w, D, index)
@@ -282,7 +284,8 @@ def norm_gate_resid_(resid: torch.Tensor, y=None, post=None, post_w=None, post_b
     elif out == "bf16":
         h = torch.empty(M, D, device=resid.device, dtype=b16)
     args = _lib.NORM_ARGS.pack(
-        resid.data_ptr(), 0 if y is None else y.data_ptr(), _lib.DT_F32 if y is not None and y.dtype is f32 else _lib.DT_BF16,
+        resid.data_ptr(), 0 if y is None else y.data_ptr(),
+        _lib.DT_F32 if y is not None and y.dtype is f32 else _lib.DT_BF16,
         NORMS[post], NORMS[pre], 0 if post_w is None else post_w.data_ptr(), 0 if post_b is None else post_b.data_ptr(),
         0 if pre_w is None else pre_w.data_ptr(), 0 if pre_b is None else pre_b.data_ptr(),
         0 if gate is None else gate.data_ptr(), 0 if shift is None else shift.data_ptr(),

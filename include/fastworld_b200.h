@@ -355,7 +355,8 @@ int fw_gemm_e4m3_block(const void* A8, const void* sa, const void* B8, const voi
  * for fp32 resid [M, D], y [M, D] (FW_BF16 or FW_F32), bf16 weights [D], fp32 gate / scale / shift [frames, D] with
  * f = row / rows_per_frame; post and pre are FW_NORM_*, fp32 statistics.  Any of the weights and gate may be
  * NULL (left out), shift and scale both.  y NULL: no residual update; out NULL: no second norm (not both).  out_s
- * NULL: out is bf16 [M, D]; else out, out_s are the e4m3 format above, quantised from the fp32 result. */
+ * NULL: out is bf16 [M, D]; else out, out_s are the e4m3 format above, quantised from the fp32 result.
+ * resid may be y (FW_F32), and otherwise overlaps no argument. */
 #define FW_NORM_NONE 0
 #define FW_NORM_LAYER 1
 #define FW_NORM_RMS 2

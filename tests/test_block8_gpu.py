@@ -67,7 +67,8 @@ def is_nan_code(q):
 
 # ---------------------------------------------------------------- quantiser
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
-@pytest.mark.parametrize("M,K", [(1, 1), (1, 128), (1, 1536), (3, 127), (9, 129), (257, 1283), (8, 512), (7, 516), (300, 2050),
+@pytest.mark.parametrize("M,K", [(1, 1), (1, 128), (1, 1536), (3, 127), (9, 129), (257, 1283), (8, 512), (7, 516),
+                                 (300, 2050),
                                  (1001, 640)])
 def test_quant_exact(M, K, dtype):
     from fastworld_b200 import ops
@@ -215,6 +216,48 @@ def test_gemm_infinities(M, N, K, out):
         assert torch.equal(s, rs) and torch.equal(is_nan_code(q), is_nan_code(rq))
         keep = ~is_nan_code(rq)
         assert torch.equal(q[keep], rq[keep])
+
+
+# several waves of 256 x 256 tiles on CTA pairs: rows and columns that end inside a tile, a group of scales that
+# K does not fill, rows of C that no 16-byte store can address (4500 bf16, 4503)
+@pytest.mark.parametrize("M,N,K", [(2600, 4504, 768), (2601, 4500, 769), (2640, 4503, 1400)])
+@pytest.mark.parametrize("epi", ["none", "gelu_tanh", "gelu_erf"])
+@pytest.mark.parametrize("out", ["bf16", "f32", "e4m3"])
+def test_gemm_large_epilogues(M, N, K, epi, out):
+    test_gemm_epilogues(M, N, K, epi, out)
+
+
+@pytest.mark.parametrize("out", ["f32", "e4m3"])
+def test_gemm_large_infinities(out):
+    test_gemm_infinities(2600, 4504, 768, out)
+
+
+@pytest.mark.parametrize("M,N,K", [(3, 200, 70001), (300, 520, 20000), (1000, 900, 9000)])
+def test_gemm_long_sums(M, N, K):
+    test_gemm_f32(M, N, K)
+
+
+def test_offsets_past_32_bits():
+    """The last rows of tensors of more than 2^31 elements are what they are alone."""
+    from fastworld_b200 import ops
+    M, D, last = 1100001, 2048, slice(-300, None)
+    x = torch.zeros(M, D, device="cuda", dtype=torch.bfloat16)
+    x[last] = rand(300, D, seed=1)
+    q, s = ops.quant_e4m3_block(x)
+    rq, rs = ops.quant_e4m3_block(x[last])
+    assert torch.equal(q[last], rq) and torch.equal(s[:, last], rs) and not q[:-300].any()
+    del q, s
+    resid = torch.zeros(M, D, device="cuda")
+    resid[last] = rand(300, D, seed=2, dtype=torch.float32)
+    alone = resid[last].clone()
+    ref = ops.norm_gate_resid_(alone, x[last], post="rms", pre="layer")
+    out = ops.norm_gate_resid_(resid, x, post="rms", pre="layer")
+    assert torch.equal(out[last], ref) and torch.equal(resid[last], alone) and not resid[:-300].any()
+    del out, resid, x
+    a8, sa, b8, sb = operands(M, D, 128)
+    got = ops.gemm_e4m3_block(a8, sa, b8, sb, out="f32")[last]
+    va, vb = value(a8[last], sa[:, last]), value(b8, sb)
+    assert ((got.double() - va @ vb.t()).abs() <= 132 * 2.0 ** -24 * (va.abs() @ vb.abs().t())).all()
 
 
 def test_gemm_no_rows():
