@@ -841,13 +841,15 @@ def block8(reps: int) -> None:
               f"{name}: {ms * 1e3:.2f} us/launch, {work / ms / 1e6:.0f} {unit}")
 
     xs = _rows(6, lambda i: rand(2640, 8960))
-    run("quant_e4m3_block 2640x8960", [lambda x=x: ops.quant_e4m3_block(x) for x in xs], 2640 * 8960 * (3 + 1 / 128), "GB/s")
+    run("quant_e4m3_block 2640x8960", [lambda x=x: ops.quant_e4m3_block(x) for x in xs], 2640 * 8960 * (3 + 1 / 128),
+        "GB/s")
     del xs
     for M, N, K, epi, out in ((2640, 4608, 1536, "none", "bf16"), (2640, 8960, 1536, "gelu_tanh", "e4m3"),
                               (2640, 1536, 8960, "none", "bf16"), (4680, 13824, 5120, "gelu_tanh", "bf16"),
                               (512, 1536, 4096, "gelu_tanh", "bf16"), (1, 9216, 1536, "none", "f32")):
         sets = _rows(max(2, min(24, int(2.6e8 / ((M + N) * K)) + 1)),
-                     lambda i: (*ops.quant_e4m3_block(rand(M, K)), *ops.quant_e4m3_block(rand(N, K, size=K ** -0.5)), rand(N)))
+                     lambda i: (*ops.quant_e4m3_block(rand(M, K)), *ops.quant_e4m3_block(rand(N, K, size=K ** -0.5)),
+                                rand(N)))
         run(f"gemm_e4m3_block {M}x{N}x{K} {epi} {out}",
             [lambda s=s: ops.gemm_e4m3_block(*s, epilogue=epi, out=out) for s in sets], 2.0 * M * N * K, "TFLOP/s")
         del sets
@@ -913,7 +915,8 @@ KERNELS = {"chunk": lambda a: chunk(a.chunks, a.config), "gemm": lambda a: gemm(
            "lingbot": lambda a: lingbot(a.reps), "lingbot_chunk": lambda a: lingbot_chunk(a.reps),
            "gemm_resid": lambda a: gemm_resid(a.reps), "attn": lambda a: attn(a.reps), "ln": lambda a: ln(a.reps),
            "ln14": lambda a: ln14(a.reps), "rms": lambda a: rms(a.reps), "copy": lambda a: copy(a.reps),
-           "block8": lambda a: block8(a.reps), "fp8_peak": lambda a: fp8_peak(a.reps), "gemm_vs_cublas": lambda a: gemm_vs_cublas(a.reps)}
+           "block8": lambda a: block8(a.reps), "fp8_peak": lambda a: fp8_peak(a.reps),
+           "gemm_vs_cublas": lambda a: gemm_vs_cublas(a.reps)}
 
 
 def main():

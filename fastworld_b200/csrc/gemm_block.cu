@@ -333,10 +333,10 @@ int launch_nk(const void* A8, const void* B8, const BlockGemmArgs& a, cudaStream
 }
 
 // Which kernel, tile and split: the least of a time model (us) whose constants were fitted to measured times
-// (small tiles: 70 sizes of 1 to 4000 rows, 30 to 13824 columns, 60 to 8960 of K; between the two kernels: 37 sizes, where
-// its choice is the faster one but for two, 4 and 7 % off).  Small tiles: launch, then the busiest SM's operand
-// bytes, or the latency of a CTA's chain of k-blocks, or HBM, then the exposed epilogue and the join of a split; wide
-// kernel: waves of 256 x 256 tiles, more for rows that no TMA store can address.
+// (small tiles: 70 sizes of 1 to 4000 rows, 30 to 13824 columns, 60 to 8960 of K; between the two kernels: 37
+// sizes, where its choice is the faster one but for two, 4 and 7 % off).  Small tiles: launch, then the busiest SM's
+// operand bytes, or the latency of a CTA's chain of k-blocks, or HBM, then the exposed epilogue and the join of a
+// split; wide kernel: waves of 256 x 256 tiles, more for rows that no TMA store can address.
 // Both sides, measured (us):
 //   small tiles   880 x 1536 x 8960   20.4 (split 3 ways; 30.9 unsplit)   25.5 wide
 //                 512 x 1536 x 13824  19.1                                36.5 wide
@@ -368,7 +368,8 @@ Plan make_plan(int M, int N, int num_kb, int out_dtype) {
       const double per_sm = (double)up(tiles * sp, sms), kbs = (double)up(num_kb, sp);
       const double load = per_sm * kbs * (128 + bn) * b8::BLK / 1.8e5;
       const double chain = up(tiles * sp, 2 * sms) * kbs * 0.5;
-      const double t = 1.7 + fmax(fmax(load, chain), hbm) + 0.9 * bn / 128 * per_sm + (sp == 1 ? 0.0 : bn == 128 ? 4.6 : 3.4);
+      const double join = sp == 1 ? 0.0 : bn == 128 ? 4.6 : 3.4;
+      const double t = 1.7 + fmax(fmax(load, chain), hbm) + 0.9 * bn / 128 * per_sm + join;
       if (t < least) {
         least = t;
         best = {bn, sp};

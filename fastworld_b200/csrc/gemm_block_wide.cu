@@ -16,10 +16,10 @@
 // Every wait is bounded; a wait that runs out makes both CTAs unwind.
 //
 // What bounds it: the tensor core needs 2048 cycles for four k-blocks of 256 x 256 x 128, and their issue takes
-// 2240 (270 cycles for a block's four MMAs, 100 for its wait, 60 for its commit), 0.30 us a block; with all pairs' loads
-// 0.36 us.  A call adds 4 us (first tile, last epilogue), a tile change 0.4 us.  2640 rows, bf16 result: 4608 x 1536 18.2 us
-// (2.05 PFLOP/s), 8960 x 1536 32.6 (2.2), 1536 x 8960 29.3 (2.5); 4680 x 13824 x 5120 233 us (2.8), and 271 us when it
-// repeats for seconds at the power limit.
+// 2240 (270 cycles for a block's four MMAs, 100 for its wait, 60 for its commit), 0.30 us a block; with all pairs
+// loading 0.36 us, 13 TB/s out of L2.  A call adds 4 us (first tile, last epilogue), a tile change 0.4 us.  2640 rows,
+// bf16 result: 4608 x 1536 18.2 us (2.05 PFLOP/s), 8960 x 1536 32.6 (2.2), 1536 x 8960 29.3 (2.5); 4680 x 13824 x 5120
+// 233 us (2.8), and 271 us when it repeats for seconds at the power limit.
 // Tried: tiles of 240 columns whose accumulators do not overlap (18.5 -> 20.7 us, 237 -> 260), four stages (240 ->
 // 245), a store wait and an exit barrier without release (18.5 -> 18.2; but then arrivals at a CTA that has left
 // are excluded by timing only); halves of 128 columns for a last wave that leaves pairs idle (issue takes as long

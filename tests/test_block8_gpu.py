@@ -149,7 +149,8 @@ def test_gemm_f32(M, N, K):
     assert torch.equal(out, again)
 
 
-@pytest.mark.parametrize("M,N,K", [(1, 640, 512), (40, 129, 256), (200, 384, 1280), (700, 1000, 512), (2640, 1536, 256)])
+@pytest.mark.parametrize("M,N,K", [(1, 640, 512), (40, 129, 256), (200, 384, 1280), (700, 1000, 512),
+                                   (2640, 1536, 256)])
 @pytest.mark.parametrize("epi", ["none", "gelu_tanh", "gelu_erf"])
 @pytest.mark.parametrize("out", ["bf16", "f32", "e4m3"])
 def test_gemm_epilogues(M, N, K, epi, out):
@@ -362,7 +363,8 @@ def test_norm_plain_forms():
 # ---------------------------------------------------------------- together, streams, graphs
 def _block(x, y, W, ops):
     """norm -> q/k/v-like product; feed-forward pair; norm and residual: one block's linears."""
-    h8, sh = ops.norm_gate_resid_(x, y, post="rms", gate=W["gate"], pre="layer", shift=W["shift"], scale=W["scale"], out="e4m3")
+    h8, sh = ops.norm_gate_resid_(x, y, post="rms", gate=W["gate"], pre="layer", shift=W["shift"], scale=W["scale"],
+                                  out="e4m3")
     u8, su = ops.gemm_e4m3_block(h8, sh, *W["up"], W["b1"], epilogue="gelu_tanh", out="e4m3")
     v = ops.gemm_e4m3_block(u8, su, *W["down"], W["b2"])
     return ops.norm_gate_resid_(x, v, post="layer", gate=W["gate"], pre="rms")
@@ -371,7 +373,8 @@ def _block(x, y, W, ops):
 def _weights(D, F):
     from fastworld_b200 import ops
     return {"gate": rand(1, D, seed=1, dtype=torch.float32), "shift": rand(1, D, seed=2, dtype=torch.float32),
-            "scale": rand(1, D, seed=3, dtype=torch.float32), "b1": rand(F, seed=4, size=0.1), "b2": rand(D, seed=5, size=0.1),
+            "scale": rand(1, D, seed=3, dtype=torch.float32), "b1": rand(F, seed=4, size=0.1),
+            "b2": rand(D, seed=5, size=0.1),
             "up": ops.quant_e4m3_block(rand(F, D, seed=6, size=D ** -0.5)),
             "down": ops.quant_e4m3_block(rand(D, F, seed=7, size=F ** -0.5))}
 
@@ -441,7 +444,8 @@ def test_refusals():
            lambda: ops.gemm_e4m3_block(a8, sa, b8, sb, v[:100]), lambda: ops.gemm_e4m3_block(a8.cpu(), sa, b8, sb),
            lambda: ops.gemm_e4m3_block(a8, sa.cpu(), b8, sb), lambda: ops.gemm_e4m3_block(a8, sa, b8, sb, out="e5m2"),
            lambda: ops.gemm_e4m3_block(a8, sa, b8, sb, epilogue="silu"),
-           lambda: ops.norm_gate_resid_(y), lambda: ops.norm_gate_resid_(x, y[:3]), lambda: ops.norm_gate_resid_(x, y.half()),
+           lambda: ops.norm_gate_resid_(y), lambda: ops.norm_gate_resid_(x, y[:3]),
+           lambda: ops.norm_gate_resid_(x, y.half()),
            lambda: ops.norm_gate_resid_(x, y, post="batch"), lambda: ops.norm_gate_resid_(x, y, post_w=v),
            lambda: ops.norm_gate_resid_(x, y, post_w=w[:100]), lambda: ops.norm_gate_resid_(x, y, gate=w),
            lambda: ops.norm_gate_resid_(x, y, gate=v.view(1, -1), rows_per_frame=3),
