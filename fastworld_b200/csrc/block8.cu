@@ -8,21 +8,22 @@ namespace fw {
 
 namespace {
 
-// Four consecutive columns of a row as loaded; VEC: one access, at an address aligned to it.
-template <typename T, bool VEC>
+// A lane's four columns of a block of 128.  VEC: adjacent ones, one access, where rows start at addresses aligned
+// to it.  Else every STEP-th one by scalar accesses.
+template <typename T, bool VEC, int STEP>
 struct Four {
   float v[4];
-  __device__ __forceinline__ void load(const T* row, int c, int K) {   // columns [c, c + 4), zeros behind K
+  __device__ __forceinline__ void load(const T* row, int c, int K) {   // zeros behind K
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = c + i < K ? static_cast<float>(row[c + i]) : 0.f;
+    for (int i = 0; i < 4; ++i) v[i] = c + i * STEP < K ? static_cast<float>(row[c + i * STEP]) : 0.f;
   }
   __device__ __forceinline__ void get(float2 (&o)[2]) const {
     o[0] = make_float2(v[0], v[1]);
     o[1] = make_float2(v[2], v[3]);
   }
 };
-template <>
-struct Four<float, true> {
+template <int STEP>
+struct Four<float, true, STEP> {
   float4 u;
   __device__ __forceinline__ void load(const float* row, int c, int K) {
     u = c < K ? *reinterpret_cast<const float4*>(row + c) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -32,8 +33,8 @@ struct Four<float, true> {
     o[1] = make_float2(u.z, u.w);
   }
 };
-template <>
-struct Four<__nv_bfloat16, true> {
+template <int STEP>
+struct Four<__nv_bfloat16, true, STEP> {
   uint2 u;
   __device__ __forceinline__ void load(const __nv_bfloat16* row, int c, int K) {
     u = c < K ? *reinterpret_cast<const uint2*>(row + c) : make_uint2(0u, 0u);
@@ -43,8 +44,8 @@ struct Four<__nv_bfloat16, true> {
     o[1] = unpack_bf16(u.y);
   }
 };
-template <>
-struct Four<__half, true> {
+template <int STEP>
+struct Four<__half, true, STEP> {
   uint2 u;
   __device__ __forceinline__ void load(const __half* row, int c, int K) {
     u = c < K ? *reinterpret_cast<const uint2*>(row + c) : make_uint2(0u, 0u);
@@ -72,7 +73,7 @@ __global__ void __launch_bounds__(QROWS * 32) quant_block_kernel(const T* __rest
   const long long row = (long long)blockIdx.x * QROWS + (threadIdx.x >> 5);
   if (row >= M) return;
   const int Kp = b8::padded(K), c0 = g * b8::GRP * b8::BLK + lane * 4;
-  Four<T, VEC> in[b8::GRP];
+  Four<T, VEC, 1> in[b8::GRP];
 #pragma unroll
   for (int b = 0; b < b8::GRP; ++b) in[b].load(x + (size_t)row * K, c0 + b * b8::BLK, K);
   uint32_t word = b8::ONES;
@@ -137,7 +138,13 @@ __device__ __forceinline__ float row_sum(float v, float* slot, int warp, int lan
 
 // Normalises x in place: fp32 mean and, about it, fp32 mean square (two sums, no cancellation).  Pairs of
 // columns on the packed fp32 pipe: with few rows per SM in flight, instructions count as much as bytes.
-template <int W, int NB>
+// From one of a lane's four columns of a block to the next: where a row's addresses are not aligned to
+// four elements, a lane takes every 32nd column, so that each of the warp's scalar accesses is contiguous
+// (2640 x 1535 14.0 us; scalar accesses of four adjacent columns 27.0).
+template <bool VEC>
+constexpr int column_step = VEC ? 1 : 32;
+
+template <bool VEC, int W, int NB>
 __device__ __forceinline__ void norm_row(float2 (&x)[NB][2], int kind, float eps, int D, int c0, float* slots, int warp,
                                          int lane) {
   const float inv_d = 1.f / (float)D;
@@ -157,9 +164,9 @@ __device__ __forceinline__ void norm_row(float2 (&x)[NB][2], int kind, float eps
       for (int b = 0; b < NB; ++b) {
         const int c = c0 + b * b8::BLK;
         if (c >= D) x[b][0].x = 0.f;
-        if (c + 1 >= D) x[b][0].y = 0.f;
-        if (c + 2 >= D) x[b][1].x = 0.f;
-        if (c + 3 >= D) x[b][1].y = 0.f;
+        if (c + column_step<VEC> >= D) x[b][0].y = 0.f;
+        if (c + 2 * column_step<VEC> >= D) x[b][1].x = 0.f;
+        if (c + 3 * column_step<VEC> >= D) x[b][1].y = 0.f;
       }
     }
   }
@@ -177,24 +184,28 @@ __device__ __forceinline__ void norm_row(float2 (&x)[NB][2], int kind, float eps
 
 // Warps that an SM has to hold, which sets the registers: 48 of them (about 40 registers) measured 15.7 us at
 // 2640 x 1536, 40 11.7, 32 11.5 (but 23.7 against 22.4 at 6032 rows), as many as the compiler's 67 registers allow
-// 12.0; at 4680 x 5120 30 warps 56.3 us, 20 (69 registers) 63.7, 40 97.
-constexpr int norm_warps(int NB) { return NB <= 3 ? 40 : NB == 4 ? 32 : 16; }
+// 12.0; at 4680 x 5120 30 warps 56.3 us, 20 (69 registers) 63.7, 40 97.  Scalar accesses take more registers: 2640 x
+// 1535 40 warps 18.8 us, 32 14.0, 24 15.0; 4680 x 4799 30 warps 97, 20 75.6.
+constexpr int norm_warps(bool VEC, int NB) {
+  return VEC ? (NB <= 3 ? 40 : NB == 4 ? 32 : 16) : (NB <= 3 ? 32 : NB == 4 ? 20 : 16);
+}
 
 template <typename Y, bool VEC, int W, int NB>
-__global__ void __launch_bounds__(W * 32, norm_warps(NB) / W) norm_gate_resid_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(W * 32, norm_warps(VEC, NB) / W) norm_gate_resid_kernel(const NormArgs a) {
   pdl_trigger();
   pdl_wait();
   __shared__ float slots[4 * W];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int row = blockIdx.x, D = a.D;
-  const int b0 = warp * NB, c0 = b0 * b8::BLK + lane * 4;
+  const int b0 = warp * NB, c0 = b0 * b8::BLK + (VEC ? lane * 4 : lane);
+  constexpr int STEP = column_step<VEC>;
   const size_t frame = (size_t)(row / a.rows_per_frame) * D;
   float* xr = a.resid + (size_t)row * D;
   // A parameter's loads for all blocks are issued together, several parameters' before one is used: with
   // one block after the other, each waited for its own.  The branch's parameters are asked for before the first
   // sum, the output's after the last one (earlier, their registers would cost rows in flight).
-  Four<__nv_bfloat16, VEC> w[NB];
-  Four<float, VEC> f[NB], f2[NB];
+  Four<__nv_bfloat16, VEC, STEP> w[NB];
+  Four<float, VEC, STEP> f[NB], f2[NB];
   auto fetch = [&](auto& v, const auto* base) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) v[b].load(base, c0 + b * b8::BLK, D);
@@ -217,18 +228,18 @@ __global__ void __launch_bounds__(W * 32, norm_warps(NB) / W) norm_gate_resid_ke
       v[b][1] = __fadd2_rn(v[b][1], p[1]);
     }
   };
-  Four<float, VEC> xin[NB];
+  Four<float, VEC, STEP> xin[NB];
   fetch(xin, xr);
   float2 x[NB][2];
   if (a.y) {
-    Four<Y, VEC> yin[NB];
+    Four<Y, VEC, STEP> yin[NB];
     fetch(yin, static_cast<const Y*>(a.y) + (size_t)row * D);
     if (a.post_w) fetch(w, a.post_w);
     if (a.gate) fetch(f, a.gate + frame);
     float2 y[NB][2];
 #pragma unroll
     for (int b = 0; b < NB; ++b) yin[b].get(y[b]);
-    if (a.post != FW_NORM_NONE) norm_row<W, NB>(y, a.post, a.eps, D, c0, slots, warp, lane);
+    if (a.post != FW_NORM_NONE) norm_row<VEC, W, NB>(y, a.post, a.eps, D, c0, slots, warp, lane);
     if (a.post_w) mul(y, w);
     if (a.post_b) {
       fetch(w, a.post_b);
@@ -246,9 +257,9 @@ __global__ void __launch_bounds__(W * 32, norm_warps(NB) / W) norm_gate_resid_ke
         if (c < D) *reinterpret_cast<float4*>(xr + c) = make_float4(x[b][0].x, x[b][0].y, x[b][1].x, x[b][1].y);
       } else {
         if (c < D) xr[c] = x[b][0].x;
-        if (c + 1 < D) xr[c + 1] = x[b][0].y;
-        if (c + 2 < D) xr[c + 2] = x[b][1].x;
-        if (c + 3 < D) xr[c + 3] = x[b][1].y;
+        if (c + STEP < D) xr[c + STEP] = x[b][0].y;
+        if (c + 2 * STEP < D) xr[c + 2 * STEP] = x[b][1].x;
+        if (c + 3 * STEP < D) xr[c + 3 * STEP] = x[b][1].y;
       }
     }
   } else {
@@ -256,7 +267,7 @@ __global__ void __launch_bounds__(W * 32, norm_warps(NB) / W) norm_gate_resid_ke
     for (int b = 0; b < NB; ++b) xin[b].get(x[b]);
   }
   if (!a.out) return;
-  if (a.pre != FW_NORM_NONE) norm_row<W, NB>(x, a.pre, a.eps, D, c0, slots + 2 * W, warp, lane);
+  if (a.pre != FW_NORM_NONE) norm_row<VEC, W, NB>(x, a.pre, a.eps, D, c0, slots + 2 * W, warp, lane);
   if (a.pre_w) fetch(w, a.pre_w);
   if (a.scale) {
     fetch(f, a.scale + frame);
@@ -286,7 +297,13 @@ __global__ void __launch_bounds__(W * 32, norm_warps(NB) / W) norm_gate_resid_ke
       if (blk * b8::BLK < Dp) {   // zeros behind D: every parameter reads as zero there
         uint32_t eb;
         const uint32_t code = b8::encode_block(x[b], eb);
-        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.out) + (size_t)row * Dp + c) = code;
+        uint8_t* o = static_cast<uint8_t*>(a.out) + (size_t)row * Dp + c;
+        if (VEC) {
+          *reinterpret_cast<uint32_t*>(o) = code;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i * STEP] = (uint8_t)(code >> (8 * i));
+        }
         if (lane == 0) a.out_s[((size_t)(blk / b8::GRP) * a.M + row) * b8::GRP + blk % b8::GRP] = (uint8_t)eb;
       }
     } else if (VEC) {
@@ -296,9 +313,9 @@ __global__ void __launch_bounds__(W * 32, norm_warps(NB) / W) norm_gate_resid_ke
     } else {
       __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.out) + (size_t)row * D;
       if (c < D) o[c] = __float2bfloat16_rn(x[b][0].x);
-      if (c + 1 < D) o[c + 1] = __float2bfloat16_rn(x[b][0].y);
-      if (c + 2 < D) o[c + 2] = __float2bfloat16_rn(x[b][1].x);
-      if (c + 3 < D) o[c + 3] = __float2bfloat16_rn(x[b][1].y);
+      if (c + STEP < D) o[c + STEP] = __float2bfloat16_rn(x[b][0].y);
+      if (c + 2 * STEP < D) o[c + 2 * STEP] = __float2bfloat16_rn(x[b][1].x);
+      if (c + 3 * STEP < D) o[c + 3 * STEP] = __float2bfloat16_rn(x[b][1].y);
     }
   }
   if (a.out_s && threadIdx.x == 0)   // places behind the last block
@@ -306,19 +323,32 @@ __global__ void __launch_bounds__(W * 32, norm_warps(NB) / W) norm_gate_resid_ke
       a.out_s[((size_t)(blk / b8::GRP) * a.M + row) * b8::GRP + blk % b8::GRP] = 127;
 }
 
-// Warps per row and blocks per warp by the row's width, each at the registers that the compiler gave it: at 1536
-// columns 4 x 3 measured 11.1 us for 2640 rows, 6 x 2 12.2, 12 x 1 16.1 and 2 x 6 12.1; at 5120 columns 10 x 4
-// 66.8 us for 4680 rows, 14 x 3 65.9, 8 x 6 68.4, 20 x 2 105.
+// Warps per row and blocks per warp (W x NB) by the row's width, as close a fit as there is: blocks that a warp
+// holds behind the row cost registers and idle lanes.  Measured for 6032 rows: 384 columns 2 x 2 9.4 us, 4 x 1 10.6;
+// 768 columns 3 x 2 13.1, 4 x 2 14.6, 4 x 3 17.4; 1152 columns 3 x 3 18.4, 4 x 3 19.9; for 4680 rows: 2560 columns
+// 7 x 3 31.2, 8 x 3 34.1; 4096 columns 8 x 4 45.4, 11 x 3 49.9, 10 x 4 52.2; 6144 columns 16 x 3 72.8, 12 x 4 72.8 (but 24.9
+// and 30.8 for 1000 rows of 6143), 16 x 4 83.2.  Fewer blocks per warp make more warps wait for a row's sums: 1536
+// columns 4 x 3 11.1 for 2640 rows, 6 x 2 12.2, 12 x 1 16.1; 5120 columns 10 x 4 66.8 for 4680 rows, 20 x 2 105 (these
+// before the registers were set).
 template <typename Y, bool VEC>
 int norm_launch(const NormArgs& a, cudaStream_t s) {
   const int nb = b8::blocks(a.D);
   auto go = [&](auto kern, int warps) {
     return launch_k(kern, dim3(a.M), dim3(warps * 32), 0, s, a) == cudaSuccess ? FW_OK : FW_ECUDA;
   };
-  if (nb <= 4) return go(norm_gate_resid_kernel<Y, VEC, 4, 1>, 4);
+  if (nb <= 2) return go(norm_gate_resid_kernel<Y, VEC, 2, 1>, 2);
+  if (nb <= 4) return go(norm_gate_resid_kernel<Y, VEC, 2, 2>, 2);
+  if (nb <= 6) return go(norm_gate_resid_kernel<Y, VEC, 3, 2>, 3);
+  if (nb <= 8) return go(norm_gate_resid_kernel<Y, VEC, 4, 2>, 4);
+  if (nb <= 9) return go(norm_gate_resid_kernel<Y, VEC, 3, 3>, 3);
   if (nb <= 12) return go(norm_gate_resid_kernel<Y, VEC, 4, 3>, 4);
+  if (nb <= 15) return go(norm_gate_resid_kernel<Y, VEC, 5, 3>, 5);
+  if (nb <= 18) return go(norm_gate_resid_kernel<Y, VEC, 6, 3>, 6);
+  if (nb <= 21) return go(norm_gate_resid_kernel<Y, VEC, 7, 3>, 7);
   if (nb <= 24) return go(norm_gate_resid_kernel<Y, VEC, 8, 3>, 8);
+  if (nb <= 32) return go(norm_gate_resid_kernel<Y, VEC, 8, 4>, 8);
   if (nb <= 40) return go(norm_gate_resid_kernel<Y, VEC, 10, 4>, 10);
+  if (nb <= 48) return go(norm_gate_resid_kernel<Y, VEC, 16, 3>, 16);
   if (nb <= 64) return go(norm_gate_resid_kernel<Y, VEC, 16, 4>, 16);
   return go(norm_gate_resid_kernel<Y, VEC, 16, 8>, 16);
 }

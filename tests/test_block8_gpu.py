@@ -340,6 +340,15 @@ def test_norm_gate_resid(M, D, rpf, post, pre, ydt, out):
         assert (s.int() - rs.int()).abs().max() <= 1 and (s != rs).float().mean() < 0.02
 
 
+# every number of warps per row and of blocks per warp, rows aligned to four elements and not
+@pytest.mark.parametrize("D", [200, 255, 300, 512, 701, 768, 1001, 1024, 1151, 1152, 1900, 1919, 2300, 2301, 2561, 2688,
+                               3001, 4000, 4095, 5119, 6143, 6144, 8191, 8192, 9001])
+@pytest.mark.parametrize("out", ["bf16", "e4m3"])
+def test_norm_widths(D, out):
+    test_norm_gate_resid(21, D, 8, "layer", "rms", torch.bfloat16, out)
+    test_norm_gate_resid(3, D, 1, "rms", "layer", torch.float32, out)
+
+
 def test_norm_plain_forms():
     """No y: the norm alone, the residual untouched; no options: the plain residual sum."""
     from fastworld_b200 import ops
