@@ -20,22 +20,31 @@ namespace fw {
 
 // Bounded wait for a phase, for loops whose issue rate counts: one try that lets the hardware hold
 // the thread until the phase completes (up to a millisecond), and everything else out of line, so
-// that little code sits between two MMAs.
+// that little code sits between two MMAs.  CLUSTER: the phase may be completed from the other CTA of a
+// pair, whose work is observed only by an acquire at cluster scope.
+template <bool CLUSTER>
 __device__ __forceinline__ bool mbar_try_held(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
-      : "memory");
+#define FW_TRY(SCOPE)                                                           \
+  asm volatile(                                                                 \
+      "{\n\t.reg .pred p;\n\t"                                                  \
+      "mbarrier.try_wait.parity.acquire." SCOPE ".shared::cta.b64 p, [%1], %2, %3;\n\t" \
+      "selp.u32 %0, 1, 0, p;\n\t}\n"                                           \
+      : "=r"(ok)                                                                \
+      : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)                          \
+      : "memory")
+  if constexpr (CLUSTER)
+    FW_TRY("cluster");
+  else
+    FW_TRY("cta");
+#undef FW_TRY
   return ok != 0;
 }
+template <bool CLUSTER>
 static __device__ __noinline__ bool wait_again(uint64_t* bar, uint32_t parity, volatile int* abort) {
   const uint64_t t0 = globaltimer();
   for (;;) {
-    if (mbar_try_held(bar, parity)) return true;
+    if (mbar_try_held<CLUSTER>(bar, parity)) return true;
     if (*abort) return false;
     if (globaltimer() - t0 > FW_WAIT_LIMIT_NS) {
       *abort = 1;
@@ -43,8 +52,9 @@ static __device__ __noinline__ bool wait_again(uint64_t* bar, uint32_t parity, v
     }
   }
 }
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool wait_on(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  return mbar_try_held(bar, parity) || wait_again(bar, parity, abort);
+  return mbar_try_held<CLUSTER>(bar, parity) || wait_again<CLUSTER>(bar, parity, abort);
 }
 
 namespace b8 {

@@ -8,6 +8,7 @@
 //   warp 2      exponent words of A's 128 rows and of all 256 rows of B to this CTA's shared memory, a group of
 //               512 of K at a time, in the order that the copy reads;
 //   warp 3      even CTA: copies them to the Tensor Memory of both (tcgen05.cp), two buffers of a group each;
+//               odd CTA: tells the even one that its group is there;
 //   warps 4-11  epilogue: lane quarter w % 4, column half (w - 4) / 4.
 // Tensor Memory has 512 columns; two accumulators of 256 and the 24 of the scales do not
 // fit side by side, so the accumulators overlap by 32 columns: even tiles at [0, 256), odd ones at [224, 480),
@@ -46,14 +47,13 @@ constexpr uint32_t SF_COL = 480, SF_STRIDE = 16;
 static_assert(SMEM <= 232448, "shared memory of a CTA");
 }  // namespace wide
 
-// Arrive on an mbarrier of either CTA, given by its shared::cluster address, without a release at cluster scope:
-// that waits for all that the thread has in flight, 0.6-1 us at every tile change and every group of scales
-// (2640 x 8960 x 1536 with GELU to e4m3 40.3 -> 34.9 us without it).  No thread of the other CTA reads what was
-// written before these arrivals.  They announce that Tensor Memory reads are complete (tcgen05.wait::ld), or that
-// this CTA's own shared memory holds scales, which its own tensor core reads: every lane's fence.proxy.async,
-// which completes the lane's writes towards that reader, comes before the arrival.
-__device__ __forceinline__ void mbar_arrive_either(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+// Arrive on an mbarrier of either CTA, given by its shared::cluster address, after reads of Tensor Memory: the
+// reads are complete (tcgen05.wait::ld) and ordered before what the waiting thread issues by the tcgen05 fences on
+// both sides (before_thread_sync here, after_thread_sync behind its wait); an arrival between them need not
+// order anything else, and one that does (release) waits for all that the thread has in flight, 0.6-1 us at
+// every tile change.
+__device__ __forceinline__ void mbar_arrive_tmem_read(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
 // Rows of C leave through a warp's 4 KB box: 32 rows of 128 bytes, 128-byte swizzle, one TMA store
@@ -96,7 +96,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + BAR_OFF);
   uint64_t* empty = full + STAGES;
-  uint64_t* sf_full = empty + STAGES;    // [SF_RING] a group's exponents are in both CTAs' shared memory, even CTA's
+  uint64_t* sf_full = empty + STAGES;    // [SF_RING] a group's exponents are in shared memory: the odd CTA's in
+                                         // its own; the even CTA's: in both
   uint64_t* sf_free = sf_full + SF_RING; // [SF_RING] ... are copied to Tensor Memory
   uint64_t* tfull = sf_free + SF_RING;   // [2] accumulator of an even / odd tile complete
   uint64_t* tfree = tfull + 2;           // [1] the shared columns of the last tile are read, even CTA's
@@ -118,7 +119,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
     }
     for (int b = 0; b < SF_RING; ++b) {
       mbar_init(sf_free + b, 1);
-      mbar_init(sf_full + b, 2);   // one arrival per warp: those of all lanes queue up on the barrier
+      mbar_init(sf_full + b, rank == 0 ? 2 : 1);   // one arrival per warp: those of all lanes queue up on the barrier
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(tfull + b, 1);
@@ -152,7 +153,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
         const int m = (t % num_m) * BM + (int)rank * HALF, n = (t / num_m) * BN + (int)rank * HALF;
         for (int kb = 0; kb < num_kb; ++kb, ++cnt) {
           const uint32_t stage = cnt % STAGES;
-          ok = wait_on(empty + stage, ((cnt / STAGES) & 1u) ^ 1u, abort_flag);
+          ok = wait_on<true>(empty + stage, ((cnt / STAGES) & 1u) ^ 1u, abort_flag);
           if (!ok) break;
           if (rank == 0) mbar_arrive_expect_tx(full + stage, 2 * STAGE);
           uint8_t* dst = smem + stage * STAGE;
@@ -182,11 +183,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
           const uint32_t sf = tmem + SF_COL + buf * SF_STRIDE;
           uint32_t id = idesc_mx8(BM, BN);
           // a tile's first MMA: tile it - 1's shared columns have been read, and all of tile it - 2
-          if (!accumulate && it > 0) ok = wait_on(tfree, (it - 1) & 1u, abort_flag);
+          if (!accumulate && it > 0) ok = wait_on<true>(tfree, (it - 1) & 1u, abort_flag);
           if (!ok) break;
           const int n = min(left, b8::GRP);
           for (int k = 0; k < n; ++k) {
-            ok = wait_on(full + stage, phase, abort_flag);
+            ok = wait_on<true>(full + stage, phase, abort_flag);
             if (!ok) break;
             tc_fence_after();
             umma_mx8_block<2>(one, d, desc, desc + (OP_BYTES >> 4), id, sf, sf + 4, accumulate);
@@ -223,7 +224,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
       const uint32_t sf_smem = smem_u32(smem + SF_OFF);
       for (uint32_t grp = 0; grp < groups; ++grp) {
         const uint32_t slot = grp % SF_RING, buf = grp & 1u;
-        if (!wait_on(sf_full + slot, (grp / SF_RING) & 1u, abort_flag)) break;
+        if (!wait_on<true>(sf_full + slot, (grp / SF_RING) & 1u, abort_flag)) break;
         if (!wait_on(sf_used + buf, ((grp >> 1) & 1u) ^ 1u, abort_flag)) break;
         tc_fence_after();
 #pragma unroll
@@ -234,9 +235,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
       if (one) umma_commit_pair(smem_u32(drain + 1));
       volatile int no_abort = 0;
       mbar_wait(drain + 1, 0, &no_abort, nullptr, DEV_TIMEOUT_DRAIN);
+    } else if (lane == 0) {
+      // This CTA's groups announced to the even CTA's copier.  The release at cluster scope that its scales need
+      // waits for all that the thread has in flight: 0.6-1 us a group for warp 2 with the next group's loads
+      // (2640 x 8960 x 1536 with GELU to e4m3 40.3 us instead of 34.9), little for a thread that loads nothing.
+      const uint32_t sf_full0 = mapa_cluster(sf_full, 0);
+      for (uint32_t grp = 0; grp < groups; ++grp) {
+        const uint32_t slot = grp % SF_RING;
+        if (!wait_on(sf_full + slot, (grp / SF_RING) & 1u, abort_flag)) break;
+        mbar_arrive_cluster(sf_full0 + 8u * slot);
+      }
     }
   } else if (warp == 2) {
-    const uint32_t sf_full0 = mapa_cluster(sf_full, 0);
     // A group is fetched before the last one is stored: the loads queue behind the tiles' traffic (fetched two
     // groups ahead, 2640 x 4608 x 1536 takes 18.9 us instead of 18.6).
     uint32_t w[12], next[12];
@@ -261,20 +271,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
     for (uint32_t grp = 0; grp < groups; ++grp) {
       fetch(next);
       const uint32_t slot = grp % SF_RING;
-      ok = __all_sync(0xffffffffu, wait_on(sf_free + slot, ((grp / SF_RING) & 1u) ^ 1u, abort_flag));
+      ok = __all_sync(0xffffffffu, wait_on<true>(sf_free + slot, ((grp / SF_RING) & 1u) ^ 1u, abort_flag));
       if (!ok) break;
       uint4* dst = reinterpret_cast<uint4*>(smem + SF_OFF + slot * SF_BYTES);
 #pragma unroll
       for (int c = 0; c < 3; ++c) dst[32 * c + lane] = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive_either(sf_full0 + 8u * slot);
+      if (lane == 0) mbar_arrive(sf_full + slot);
 #pragma unroll
       for (int c = 0; c < 12; ++c) w[c] = next[c];
     }
     // the last copies' arrivals from the even CTA have come: none is under way to this CTA at exit
     for (uint32_t grp = groups < SF_RING ? 0 : groups - SF_RING; grp < groups && ok; ++grp)
-      ok = wait_on(sf_free + grp % SF_RING, (grp / SF_RING) & 1u, abort_flag);
+      ok = wait_on<true>(sf_free + grp % SF_RING, (grp / SF_RING) & 1u, abort_flag);
   } else if (warp >= EPI0) {
     const int q = warp & 3, h = (warp - EPI0) >> 2;
     const uint32_t tfree0 = mapa_cluster(tfree, 0);
@@ -297,7 +307,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
         *reinterpret_cast<float4*>(bias + lane * 4) = u;
       }
       __syncwarp();
-      bool ok = __all_sync(0xffffffffu, wait_on(tfull + (it & 1u), (it >> 1) & 1u, abort_flag));
+      bool ok = __all_sync(0xffffffffu, wait_on<true>(tfull + (it & 1u), (it >> 1) & 1u, abort_flag));
       if (!ok) break;
       tc_fence_after();
       const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16) + (it & 1u) * SHIFT + (uint32_t)(h * 128);
@@ -329,7 +339,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
         tmem_ld_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_either(tfree0);
+        if (lane == 0) mbar_arrive_tmem_read(tfree0);
         scan(keep, first * 32);
 #pragma unroll 1
         for (int j = 1; j < 4; ++j) {
@@ -397,7 +407,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
         tmem_ld_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_either(tfree0);
+        if (lane == 0) mbar_arrive_tmem_read(tfree0);
 #pragma unroll 1
         for (int j = 0; j < 4; ++j) {
           const int c = first + dir * j;
