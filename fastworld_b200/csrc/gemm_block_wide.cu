@@ -183,7 +183,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
           const uint32_t sf = tmem + SF_COL + buf * SF_STRIDE;
           uint32_t id = idesc_mx8(BM, BN);
           // a tile's first MMA: tile it - 1's shared columns have been read, and all of tile it - 2
-          if (!accumulate && it > 0) ok = wait_on<true>(tfree, (it - 1) & 1u, abort_flag);
+          if (ok && !accumulate && it > 0) ok = wait_on<true>(tfree, (it - 1) & 1u, abort_flag);
           if (!ok) break;
           const int n = min(left, b8::GRP);
           for (int k = 0; k < n; ++k) {

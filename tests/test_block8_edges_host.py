@@ -28,3 +28,16 @@ def test_waits_for_another_cta_are_at_cluster_scope():
     for scope, bar in waits:
         if bar in ("empty", "full", "tfull", "tfree"):
             assert scope, bar
+
+
+def test_no_wait_hides_the_one_before():
+    """A wait that ran out ends the loop: its result is looked at before the next wait's takes its place."""
+    for name in ("gemm_block.cu", "gemm_block_wide.cu"):
+        src = source(name)
+        at = [m for m in re.finditer(r"[^\n]*\bok = (?:__all_sync\([^,]*, )?wait_on", src)]
+        assert len(at) >= 4
+        for one, two in zip(at, at[1:]):
+            if "bool ok" in two.group():      # another role's
+                continue
+            between = src[one.end():two.end()]
+            assert "!ok" in between or "if (ok" in two.group(), (name, two.group())
