@@ -146,6 +146,19 @@ __device__ __forceinline__ float2 activate2(float2 v) {
   return v;
 }
 
+// Abort flag of CTA `lane` of a cluster of `ranks`, 0 for lanes without one.  Behind a cluster barrier that follows all of
+// the ranks' waits, a vote over it tells every warp of every rank the same: whether all of them staged their part.
+__device__ __forceinline__ int cluster_abort_flag(const volatile int* flag, int ranks) {
+  const int lane = threadIdx.x & 31;
+  int v = 0;
+  if (lane < ranks)
+    asm volatile("ld.shared::cluster.b32 %0, [%1];"
+                 : "=r"(v)
+                 : "r"(mapa_cluster(const_cast<const int*>(flag), (uint32_t)lane))
+                 : "memory");
+  return v;
+}
+
 // gemm_block_wide.cu: persistent kernel for large problems.
 int gemm_block_wide_launch(const void* A8, const void* B8, const BlockGemmArgs& a, cudaStream_t s);
 

@@ -245,7 +245,9 @@ __global__ void __launch_bounds__(nk::THREADS)
     cluster_sync();   // every rank's partial is staged
   else
     __syncthreads();
-  if (__all_sync(0xffffffffu, !*abort_flag)) {
+  // Nothing is written where a wait ran out, nor, in a split, where another rank's did: its part is not staged.
+  const int gave_up = splits > 1 ? cluster_abort_flag(abort_flag, splits) : *abort_flag;
+  if (splits > 1 || __all_sync(0xffffffffu, !gave_up)) {
     float bias[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) bias[i] = __uint_as_float((uint32_t)bias_bits[i] << 16);
@@ -268,6 +270,7 @@ __global__ void __launch_bounds__(nk::THREADS)
 #pragma unroll
         for (int k = 0; k < nk::MAX_SPLITS; ++k)
           if (k < splits) u[k] = ld_cluster4(mapa_cluster(st + r * 128, (uint32_t)k));
+        if (__any_sync(0xffffffffu, gave_up)) break;   // looked at here, the flags' way is hidden behind the partials'
 #pragma unroll
         for (int k = 1; k < nk::MAX_SPLITS; ++k)
           if (k < splits) u[0].x += u[k].x, u[0].y += u[k].y, u[0].z += u[k].z, u[0].w += u[k].w;

@@ -10,8 +10,13 @@
 //     of a two-rank group whose "rank 1" buffers are this GPU's own memory and which nobody
 //     plays: both of its waits for rank 1's epoch flags run out after `limit_ns`, record
 //     DEV_TIMEOUT_PEER, and the kernel completes without the missing data.
+//   which 2 (split product): two clusters of CTAs do as the ranks of a split block-scaled product (gemm_block.cu): each
+//     waits for its part, then all meet at a cluster barrier and look at one another's abort flags.  One rank of the first
+//     cluster waits on an mbarrier that nothing completes; every warp of every rank of that cluster must see it, and no
+//     warp of the other cluster.
 // Nothing here faults: every access is in the buffers the host carves from `scratch`.
 #include "../../include/fastworld_b200.h"
+#include "fw_gemm_block.cuh"
 #include "fw_internal.h"
 #include "fw_ptx.cuh"
 #include "fw_tp.h"
@@ -55,6 +60,30 @@ __global__ void __launch_bounds__(128) mbar_timeout_kernel(uint64_t limit_ns, in
   }
 }
 
+constexpr int kSplitRanks = 4, kSplitLate = 2;   // the rank whose part never comes
+
+__global__ void __cluster_dims__(kSplitRanks, 1, 1) __launch_bounds__(64)
+    split_timeout_kernel(uint64_t limit_ns, int* status, int* outcome) {
+  pdl_wait();
+  __shared__ __align__(8) uint64_t bar;
+  __shared__ int abort_flag;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (threadIdx.x == 0) {
+    mbar_init(&bar, 1);
+    fence_mbar_init();
+    abort_flag = 0;
+  }
+  __syncthreads();
+  if (threadIdx.x == 32) {
+    if (blockIdx.x != kSplitLate) mbar_arrive(&bar);
+    mbar_wait(&bar, 0, &abort_flag, status, DEV_TIMEOUT_TEST, limit_ns);
+  }
+  cluster_sync();
+  const bool gave_up = __any_sync(0xffffffffu, cluster_abort_flag(&abort_flag, kSplitRanks));
+  if (lane == 0) outcome[blockIdx.x * 2 + warp] = gave_up ? 2 : 1;
+  cluster_sync();   // no CTA leaves while another reads its flag
+}
+
 struct PeerScratch {
   size_t part, flags, epoch, xs, end;
 };
@@ -78,6 +107,7 @@ PeerScratch peer_layout() {
 extern "C" size_t fw_selftest_bytes(int which) {
   if (which == 0) return fw::kSelfTestCtas * 2 * sizeof(int);
   if (which == 1) return fw::peer_layout().end;
+  if (which == 2) return 2 * fw::kSplitRanks * 2 * sizeof(int);
   return 0;
 }
 
@@ -90,6 +120,11 @@ extern "C" int fw_selftest_wait(int which, unsigned long long limit_ns, void* sc
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (which == 0) {
     launch_k(mbar_timeout_kernel, kSelfTestCtas, 128, 0, s, (uint64_t)limit_ns, status,
+             reinterpret_cast<int*>(scratch));
+    return cudaGetLastError() == cudaSuccess ? 0 : FW_ECUDA;
+  }
+  if (which == 2) {
+    launch_k(split_timeout_kernel, 2 * kSplitRanks, 64, 0, s, (uint64_t)limit_ns, status,
              reinterpret_cast<int*>(scratch));
     return cudaGetLastError() == cudaSuccess ? 0 : FW_ECUDA;
   }

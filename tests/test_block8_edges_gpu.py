@@ -2,7 +2,9 @@
 import pytest
 import torch
 
-from test_block8_gpu import operands, rand, value
+from test_block8_gpu import operands, rand, value  # noqa: F401
+
+from test_failure_gpu import DEV_TIMEOUT_TEST, LIMIT_NS, gemm_still_correct, run_selftest
 
 pytestmark = pytest.mark.gpu
 
@@ -30,3 +32,12 @@ def test_wide_products_are_the_same_on_every_run(M, N, K, out):
         va, vb = value(a8, sa)[rows], value(b8, sb)
         err = (first[0][rows].double() - va @ vb.t()).abs() / (va.abs() @ vb.abs().t())
         assert err.max().item() <= (K + 4) * 2.0 ** -24
+
+
+def test_a_split_without_one_part_is_seen_by_every_rank():
+    """One rank's wait runs out: all warps of all ranks of its cluster know, none of another cluster."""
+    status, scratch, ms = run_selftest(2)
+    assert int(status[0]) == DEV_TIMEOUT_TEST
+    assert scratch[:4 * 16].view(torch.int32).tolist() == [2] * 8 + [1] * 8
+    assert LIMIT_NS / 1e6 <= ms < 1000.0
+    assert gemm_still_correct() < 6e-3

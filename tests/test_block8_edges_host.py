@@ -41,3 +41,10 @@ def test_no_wait_hides_the_one_before():
                 continue
             between = src[one.end():two.end()]
             assert "!ok" in between or "if (ok" in two.group(), (name, two.group())
+
+
+def test_a_split_joins_only_what_every_rank_staged():
+    """Partials of other ranks are added only behind a look at every rank's abort flag."""
+    src = source("gemm_block.cu")
+    load, add = src.index("ld_cluster4(mapa_cluster(st"), src.index("u[0].x += u[k].x")
+    assert "cluster_abort_flag(abort_flag, splits)" in src[:load] and "__any_sync(0xffffffffu, gave_up)" in src[load:add]
