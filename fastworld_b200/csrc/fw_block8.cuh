@@ -41,20 +41,23 @@ __device__ __forceinline__ bool mbar_try_held(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 template <bool CLUSTER>
-static __device__ __noinline__ bool wait_again(uint64_t* bar, uint32_t parity, volatile int* abort) {
+static __device__ __noinline__ bool wait_again(uint64_t* bar, uint32_t parity, volatile int* abort, int* status,
+                                               int code, uint64_t limit_ns) {
   const uint64_t t0 = globaltimer();
   for (;;) {
     if (mbar_try_held<CLUSTER>(bar, parity)) return true;
     if (*abort) return false;
-    if (globaltimer() - t0 > FW_WAIT_LIMIT_NS) {
+    if (globaltimer() - t0 > limit_ns) {
       *abort = 1;
+      record_status(status, code);
       return false;
     }
   }
 }
 template <bool CLUSTER = false>
-__device__ __forceinline__ bool wait_on(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  return mbar_try_held<CLUSTER>(bar, parity) || wait_again<CLUSTER>(bar, parity, abort);
+__device__ __forceinline__ bool wait_on(uint64_t* bar, uint32_t parity, volatile int* abort, int* status, int code,
+                                        uint64_t limit_ns = FW_WAIT_LIMIT_NS) {
+  return mbar_try_held<CLUSTER>(bar, parity) || wait_again<CLUSTER>(bar, parity, abort, status, code, limit_ns);
 }
 
 namespace b8 {

@@ -16,6 +16,7 @@ struct BlockGemmArgs {
   int splits;                  // CTAs that share a tile's k-blocks (gemm_block.cu)
   void* out;                   // bf16 / fp32 [M, N], or codes [M, Np]
   uint8_t* out_s;              // exponents of codes
+  int* status;                 // a wait that runs out records its code here, or null
 };
 
 // Instruction descriptor of kind::mxf8f6f4: e4m3 operands, both K-major, UE8M0 scales (bit 23).
@@ -146,8 +147,8 @@ __device__ __forceinline__ float2 activate2(float2 v) {
   return v;
 }
 
-// Abort flag of CTA `lane` of a cluster of `ranks`, 0 for lanes without one.  Behind a cluster barrier that follows all of
-// the ranks' waits, a vote over it tells every warp of every rank the same: whether all of them staged their part.
+// Abort flag of CTA `lane` of a cluster of `ranks`, 0 for lanes without one.  Behind a cluster barrier that follows all
+// of the ranks' waits, a vote over it tells every warp of every rank the same: whether all of them staged their part.
 __device__ __forceinline__ int cluster_abort_flag(const volatile int* flag, int ranks) {
   const int lane = threadIdx.x & 31;
   int v = 0;

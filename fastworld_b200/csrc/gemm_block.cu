@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(nk::THREADS)
       for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
         const int s = i % C::STAGES;
         const uint32_t par = (uint32_t)(i / C::STAGES) & 1u;
-        if (!wait_on(empty + s, par ^ 1u, abort_flag)) break;
+        if (!wait_on(empty + s, par ^ 1u, abort_flag, a.status, DEV_TIMEOUT_PRODUCER)) break;
         mbar_arrive_expect_tx(full + s, C::STAGE);
         tma_load_2d(smem + s * C::STAGE, &tmP, full + s, kb * b8::BLK, n0);
         tma_load_2d(smem + s * C::STAGE + C::P_BYTES, &tmQ, full + s, kb * b8::BLK, m0);
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(nk::THREADS)
       }
       volatile int no_abort = 0;   // no copy into this CTA's memory is in flight at exit
       for (int s = 0; s < C::STAGES; ++s)
-        if (used >> s & 1u) mbar_wait(full + s, last_par >> s & 1u, &no_abort, nullptr, DEV_TIMEOUT_DRAIN);
+        if (used >> s & 1u) mbar_wait(full + s, last_par >> s & 1u, &no_abort, a.status, DEV_TIMEOUT_DRAIN);
     }
   } else if (warp == 1) {
     const uint32_t one = lane == 0;
@@ -167,8 +167,9 @@ __global__ void __launch_bounds__(nk::THREADS)
     bool ok = true;
     for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
       const int s = i % C::STAGES, grp = kb / b8::GRP - kb0 / b8::GRP, buf = grp & 1;
-      if (i == 0 || kb % b8::GRP == 0) ok = wait_on(sf_full + buf, (uint32_t)(grp >> 1) & 1u, abort_flag);
-      if (ok) ok = wait_on(full + s, (uint32_t)(i / C::STAGES) & 1u, abort_flag);
+      if (i == 0 || kb % b8::GRP == 0)
+        ok = wait_on(sf_full + buf, (uint32_t)(grp >> 1) & 1u, abort_flag, a.status, DEV_TIMEOUT_MMA);
+      if (ok) ok = wait_on(full + s, (uint32_t)(i / C::STAGES) & 1u, abort_flag, a.status, DEV_TIMEOUT_MMA);
       if (!ok) break;
       tc_fence_after();
       const uint32_t desc = desc_lo(smem_u32(smem + s * C::STAGE));
@@ -180,7 +181,7 @@ __global__ void __launch_bounds__(nk::THREADS)
     }
     umma_commit_if<1>(one, done);
     volatile int no_abort = 0;
-    mbar_wait(done, 0, &no_abort, nullptr, DEV_TIMEOUT_DRAIN);
+    mbar_wait(done, 0, &no_abort, a.status, DEV_TIMEOUT_DRAIN);
   } else if (warp < 6) {
     const int q = warp & 3;   // lane quarter of Tensor Memory
     const uint32_t quarter = tmem + ((uint32_t)(q * 32) << 16);
@@ -199,7 +200,8 @@ __global__ void __launch_bounds__(nk::THREADS)
       }
       const int buf = i & 1;
       if (i >= 2) {
-        ok = __all_sync(0xffffffffu, wait_on(sf_free + buf, (uint32_t)((i - 2) >> 1) & 1u, abort_flag));
+        ok = __all_sync(0xffffffffu, wait_on(sf_free + buf, (uint32_t)((i - 2) >> 1) & 1u, abort_flag, a.status,
+                                             DEV_TIMEOUT_EPILOGUE));
         if (!ok) break;
         tc_fence_after();
       }
@@ -209,7 +211,7 @@ __global__ void __launch_bounds__(nk::THREADS)
       tc_fence_before();
       mbar_arrive(sf_full + buf);
     }
-    if (ok) ok = __all_sync(0xffffffffu, wait_on(done, 0, abort_flag));
+    if (ok) ok = __all_sync(0xffffffffu, wait_on(done, 0, abort_flag, a.status, DEV_TIMEOUT_EPILOGUE));
     if (ok) {
       // accumulator lane = column of C, column = row of C; staged as [row][128 columns]
       tc_fence_after();
@@ -389,6 +391,12 @@ Plan make_plan(int M, int N, int num_kb, int out_dtype) {
 extern "C" int fw_gemm_e4m3_block(const void* A8, const void* sa, const void* B8, const void* sb, const void* bias,
                                   void* out, void* out_s, int M, int N, int K, int epilogue, int out_dtype,
                                   void* stream) {
+  return fw_gemm_e4m3_block_status(A8, sa, B8, sb, bias, out, out_s, M, N, K, epilogue, out_dtype, nullptr, stream);
+}
+
+extern "C" int fw_gemm_e4m3_block_status(const void* A8, const void* sa, const void* B8, const void* sb,
+                                         const void* bias, void* out, void* out_s, int M, int N, int K, int epilogue,
+                                         int out_dtype, int* status, void* stream) {
   using namespace fw;
   if (M < 0 || N < 0 || K <= 0 || K > FW_BLOCK_MAX_COLS || N > FW_BLOCK_MAX_COLS) return FW_ESHAPE;
   BlockGemmArgs a;
@@ -405,7 +413,7 @@ extern "C" int fw_gemm_e4m3_block(const void* A8, const void* sa, const void* B8
     if (reinterpret_cast<uintptr_t>(p) % 16) return FW_EALIGN;
   for (const void* p : {sa, sb, (const void*)out_s})
     if (reinterpret_cast<uintptr_t>(p) % 4) return FW_EALIGN;
-  if (reinterpret_cast<uintptr_t>(bias) % 2) return FW_EALIGN;
+  if (reinterpret_cast<uintptr_t>(bias) % 2 || reinterpret_cast<uintptr_t>(status) % 4) return FW_EALIGN;
   a.M = M;
   a.N = N;
   a.K = b8::padded(K);
@@ -415,6 +423,7 @@ extern "C" int fw_gemm_e4m3_block(const void* A8, const void* sa, const void* B8
   a.out_dtype = out_dtype;
   a.out = out;
   a.out_s = static_cast<uint8_t*>(out_s);
+  a.status = status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const Plan p = make_plan(M, N, a.K / b8::BLK, out_dtype);
   a.splits = p.splits;

@@ -153,7 +153,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
         const int m = (t % num_m) * BM + (int)rank * HALF, n = (t / num_m) * BN + (int)rank * HALF;
         for (int kb = 0; kb < num_kb; ++kb, ++cnt) {
           const uint32_t stage = cnt % STAGES;
-          ok = wait_on<true>(empty + stage, ((cnt / STAGES) & 1u) ^ 1u, abort_flag);
+          ok = wait_on<true>(empty + stage, ((cnt / STAGES) & 1u) ^ 1u, abort_flag, a.status, DEV_TIMEOUT_PRODUCER);
           if (!ok) break;
           if (rank == 0) mbar_arrive_expect_tx(full + stage, 2 * STAGE);
           uint8_t* dst = smem + stage * STAGE;
@@ -164,7 +164,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
       // the MMAs consumed every stage this thread filled: no copy into this CTA is in flight at exit
       volatile int no_abort = 0;
       for (uint32_t c = cnt < STAGES ? 0 : cnt - STAGES; c < cnt; ++c)
-        mbar_wait(empty + c % STAGES, (c / STAGES) & 1u, &no_abort, nullptr, DEV_TIMEOUT_DRAIN);
+        mbar_wait(empty + c % STAGES, (c / STAGES) & 1u, &no_abort, a.status, DEV_TIMEOUT_DRAIN);
     }
   } else if (warp == 1) {
     if (rank == 0) {
@@ -179,15 +179,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
         const uint32_t d = tmem + (it & 1u) * SHIFT;
         uint32_t accumulate = 0;
         for (int left = num_kb; left > 0;) {
-          ok = wait_on(sf_free + slot, slot_phase, abort_flag);   // copied
+          ok = wait_on(sf_free + slot, slot_phase, abort_flag, a.status, DEV_TIMEOUT_MMA);   // copied
           const uint32_t sf = tmem + SF_COL + buf * SF_STRIDE;
           uint32_t id = idesc_mx8(BM, BN);
           // a tile's first MMA: tile it - 1's shared columns have been read, and all of tile it - 2
-          if (ok && !accumulate && it > 0) ok = wait_on<true>(tfree, (it - 1) & 1u, abort_flag);
+          if (ok && !accumulate && it > 0)
+            ok = wait_on<true>(tfree, (it - 1) & 1u, abort_flag, a.status, DEV_TIMEOUT_MMA);
           if (!ok) break;
           const int n = min(left, b8::GRP);
           for (int k = 0; k < n; ++k) {
-            ok = wait_on<true>(full + stage, phase, abort_flag);
+            ok = wait_on<true>(full + stage, phase, abort_flag, a.status, DEV_TIMEOUT_MMA);
             if (!ok) break;
             tc_fence_after();
             umma_mx8_block<2>(one, d, desc, desc + (OP_BYTES >> 4), id, sf, sf + 4, accumulate);
@@ -215,7 +216,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
       }
       if (one) umma_commit_pair(smem_u32(drain));   // this CTA's only: nothing arrives at a CTA that has left
       volatile int no_abort = 0;
-      mbar_wait(drain, 0, &no_abort, nullptr, DEV_TIMEOUT_DRAIN);
+      mbar_wait(drain, 0, &no_abort, a.status, DEV_TIMEOUT_DRAIN);
     }
   } else if (warp == 3) {
     if (rank == 0) {
@@ -224,8 +225,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
       const uint32_t sf_smem = smem_u32(smem + SF_OFF);
       for (uint32_t grp = 0; grp < groups; ++grp) {
         const uint32_t slot = grp % SF_RING, buf = grp & 1u;
-        if (!wait_on<true>(sf_full + slot, (grp / SF_RING) & 1u, abort_flag)) break;
-        if (!wait_on(sf_used + buf, ((grp >> 1) & 1u) ^ 1u, abort_flag)) break;
+        if (!wait_on<true>(sf_full + slot, (grp / SF_RING) & 1u, abort_flag, a.status, DEV_TIMEOUT_MMA)) break;
+        if (!wait_on(sf_used + buf, ((grp >> 1) & 1u) ^ 1u, abort_flag, a.status, DEV_TIMEOUT_MMA)) break;
         tc_fence_after();
 #pragma unroll
         for (int c = 0; c < 3; ++c)
@@ -234,7 +235,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
       }
       if (one) umma_commit_pair(smem_u32(drain + 1));
       volatile int no_abort = 0;
-      mbar_wait(drain + 1, 0, &no_abort, nullptr, DEV_TIMEOUT_DRAIN);
+      mbar_wait(drain + 1, 0, &no_abort, a.status, DEV_TIMEOUT_DRAIN);
     } else if (lane == 0) {
       // This CTA's groups announced to the even CTA's copier.  The release at cluster scope that its scales need
       // waits for all that the thread has in flight: 0.6-1 us a group for warp 2 with the next group's loads
@@ -242,7 +243,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
       const uint32_t sf_full0 = mapa_cluster(sf_full, 0);
       for (uint32_t grp = 0; grp < groups; ++grp) {
         const uint32_t slot = grp % SF_RING;
-        if (!wait_on(sf_full + slot, (grp / SF_RING) & 1u, abort_flag)) break;
+        if (!wait_on(sf_full + slot, (grp / SF_RING) & 1u, abort_flag, a.status, DEV_TIMEOUT_MMA)) break;
         mbar_arrive_cluster(sf_full0 + 8u * slot);
       }
     }
@@ -271,7 +272,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
     for (uint32_t grp = 0; grp < groups; ++grp) {
       fetch(next);
       const uint32_t slot = grp % SF_RING;
-      ok = __all_sync(0xffffffffu, wait_on<true>(sf_free + slot, ((grp / SF_RING) & 1u) ^ 1u, abort_flag));
+      ok = __all_sync(0xffffffffu, wait_on<true>(sf_free + slot, ((grp / SF_RING) & 1u) ^ 1u, abort_flag, a.status,
+                                                 DEV_TIMEOUT_PRODUCER));
       if (!ok) break;
       uint4* dst = reinterpret_cast<uint4*>(smem + SF_OFF + slot * SF_BYTES);
 #pragma unroll
@@ -284,7 +286,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
     }
     // the last copies' arrivals from the even CTA have come: none is under way to this CTA at exit
     for (uint32_t grp = groups < SF_RING ? 0 : groups - SF_RING; grp < groups && ok; ++grp)
-      ok = wait_on<true>(sf_free + grp % SF_RING, (grp / SF_RING) & 1u, abort_flag);
+      ok = wait_on<true>(sf_free + grp % SF_RING, (grp / SF_RING) & 1u, abort_flag, a.status, DEV_TIMEOUT_PRODUCER);
   } else if (warp >= EPI0) {
     const int q = warp & 3, h = (warp - EPI0) >> 2;
     const uint32_t tfree0 = mapa_cluster(tfree, 0);
@@ -307,7 +309,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
         *reinterpret_cast<float4*>(bias + lane * 4) = u;
       }
       __syncwarp();
-      bool ok = __all_sync(0xffffffffu, wait_on<true>(tfull + (it & 1u), (it >> 1) & 1u, abort_flag));
+      bool ok = __all_sync(0xffffffffu, wait_on<true>(tfull + (it & 1u), (it >> 1) & 1u, abort_flag, a.status,
+                                                      DEV_TIMEOUT_EPILOGUE));
       if (!ok) break;
       tc_fence_after();
       const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16) + (it & 1u) * SHIFT + (uint32_t)(h * 128);

@@ -76,7 +76,7 @@ __global__ void __cluster_dims__(kSplitRanks, 1, 1) __launch_bounds__(64)
   __syncthreads();
   if (threadIdx.x == 32) {
     if (blockIdx.x != kSplitLate) mbar_arrive(&bar);
-    mbar_wait(&bar, 0, &abort_flag, status, DEV_TIMEOUT_TEST, limit_ns);
+    wait_on<true>(&bar, 0, &abort_flag, status, DEV_TIMEOUT_TEST, limit_ns);   // the products' wait (fw_block8.cuh)
   }
   cluster_sync();
   const bool gave_up = __any_sync(0xffffffffu, cluster_abort_flag(&abort_flag, kSplitRanks));

@@ -179,10 +179,11 @@ def quant_e4m3_block(x: torch.Tensor):
 
 
 def gemm_e4m3_block(a8: torch.Tensor, sa: torch.Tensor, b8: torch.Tensor, sb: torch.Tensor, bias=None,
-                    epilogue: str = "none", out: str = "bf16"):
+                    epilogue: str = "none", out: str = "bf16", status: torch.Tensor = None):
     """act(A @ B^T + bias) of block-scaled e4m3 A [M, K] and B [N, K] (quant_e4m3_block), fp32 accumulation.
     epilogue: 'none', 'gelu_tanh' or 'gelu_erf'; bias bf16 [N].  out: 'bf16' or 'f32' [M, N], or 'e4m3': the
-    pair (q, s) of the result, quantised from fp32, as the next product takes it."""
+    pair (q, s) of the result, quantised from fp32, as the next product takes it.  status: int32, zeroed by the caller;
+    where a wait of the kernel runs out, its first word receives a code and parts of the result are not written."""
     if epilogue not in BLOCK_EPILOGUES:
         raise ValueError(f"epilogue: {epilogue!r}, expected one of {sorted(BLOCK_EPILOGUES)}")
     if out not in BLOCK_OUTPUTS:
@@ -201,6 +202,8 @@ def gemm_e4m3_block(a8: torch.Tensor, sa: torch.Tensor, b8: torch.Tensor, sb: to
         _refuse("sb", sb, u8, index, [groups, N, 4])
     if bias is not None and (bias.shape != (N,) or not _is(bias, torch.bfloat16, index)):
         _refuse("bias", bias, torch.bfloat16, index, [N])
+    if status is not None and (status.numel() == 0 or not _is(status, torch.int32, index)):
+        _refuse("status", status, torch.int32, index, "[at least 1]")
     code, dtype = BLOCK_OUTPUTS[out]
     if out == "e4m3":
         if N == 0:
@@ -208,8 +211,8 @@ def gemm_e4m3_block(a8: torch.Tensor, sa: torch.Tensor, b8: torch.Tensor, sb: to
         o, so = _block_empty(M, N, a8.device)
     else:
         o, so = torch.empty(M, N, device=a8.device, dtype=dtype), None
-    _on(index, lib().fw_gemm_e4m3_block, "gemm_e4m3_block", a8.data_ptr(), sa.data_ptr(), b8.data_ptr(), sb.data_ptr(),
-        ptr(bias), o.data_ptr(), ptr(so), M, N, K, BLOCK_EPILOGUES[epilogue], code)
+    _on(index, lib().fw_gemm_e4m3_block_status, "gemm_e4m3_block", a8.data_ptr(), sa.data_ptr(), b8.data_ptr(),
+        sb.data_ptr(), ptr(bias), o.data_ptr(), ptr(so), M, N, K, BLOCK_EPILOGUES[epilogue], code, ptr(status))
     return o if so is None else (o, so)
 
 

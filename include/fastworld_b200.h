@@ -349,6 +349,11 @@ int fw_quant_e4m3_block(const void* x, int dtype, int M, int K, void* q, void* s
  * is NULL otherwise).  A8, B8 and out 16-byte aligned. */
 int fw_gemm_e4m3_block(const void* A8, const void* sa, const void* B8, const void* sb, const void* bias, void* out,
                        void* out_s, int M, int N, int K, int epilogue, int out_dtype, void* stream);
+/* ... with a status word: *status (device, zeroed by the caller, or NULL) receives a code where a wait of the kernel
+ * ran out, as fw_attention's; parts of the result are then not written.  The call above leaves it out. */
+int fw_gemm_e4m3_block_status(const void* A8, const void* sa, const void* B8, const void* sb, const void* bias,
+                              void* out, void* out_s, int M, int N, int K, int epilogue, int out_dtype, int* status,
+                              void* stream);
 /* The norm after a block, its gate and the residual update, and the norm and modulation before the next:
  *   b = post(y) * post_w + post_b;   resid = resid_scale * resid + branch_scale * gate[f] * b   (in place)
  *   out = (pre(resid) * pre_w + pre_b) * (1 + scale[f]) + shift[f]

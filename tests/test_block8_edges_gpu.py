@@ -41,3 +41,18 @@ def test_a_split_without_one_part_is_seen_by_every_rank():
     assert scratch[:4 * 16].view(torch.int32).tolist() == [2] * 8 + [1] * 8
     assert LIMIT_NS / 1e6 <= ms < 1000.0
     assert gemm_still_correct() < 6e-3
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 640, 1536), (300, 512, 4096), (2640, 4608, 640)])
+@pytest.mark.parametrize("out", ["bf16", "e4m3"])
+def test_status_of_a_product(M, N, K, out):
+    from fastworld_b200 import ops
+    a8, sa, b8, sb = operands(M, N, K, seed=2)
+    status = torch.zeros(4, device="cuda", dtype=torch.int32)
+    got = ops.gemm_e4m3_block(a8, sa, b8, sb, out=out, status=status)
+    ref = ops.gemm_e4m3_block(a8, sa, b8, sb, out=out)
+    assert all(torch.equal(g, r) for g, r in (zip(got, ref) if out == "e4m3" else [(got, ref)]))
+    assert not status.any()
+    for bad in (status.long(), status.cpu(), status[:0], status[::2]):
+        with pytest.raises(ValueError, match="status"):
+            ops.gemm_e4m3_block(a8, sa, b8, sb, out=out, status=bad)

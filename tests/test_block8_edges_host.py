@@ -3,6 +3,8 @@ import glob
 import os
 import re
 
+from test_block8_host import EALIGN, EINVAL, ESHAPE, L, P  # noqa: F401
+
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "fastworld_b200", "csrc")
 
 
@@ -34,7 +36,7 @@ def test_no_wait_hides_the_one_before():
     """A wait that ran out ends the loop: its result is looked at before the next wait's takes its place."""
     for name in ("gemm_block.cu", "gemm_block_wide.cu"):
         src = source(name)
-        at = [m for m in re.finditer(r"[^\n]*\bok = (?:__all_sync\([^,]*, )?wait_on", src)]
+        at = [m for m in re.finditer(r"(?:if \([^\n]*\n)?[^\n]*\bok = (?:__all_sync\([^,]*, )?wait_on", src)]
         assert len(at) >= 4
         for one, two in zip(at, at[1:]):
             if "bool ok" in two.group():      # another role's
@@ -48,3 +50,22 @@ def test_a_split_joins_only_what_every_rank_staged():
     src = source("gemm_block.cu")
     load, add = src.index("ld_cluster4(mapa_cluster(st"), src.index("u[0].x += u[k].x")
     assert "cluster_abort_flag(abort_flag, splits)" in src[:load] and "__any_sync(0xffffffffu, gave_up)" in src[load:add]
+
+
+def test_status_entry(L):
+    """The entry with a status word turns away what the plain one does, and a word that is not aligned."""
+    def call(status=None, **kw):
+        a = dict(A=P, sa=P, B=P, sb=P, bias=P, out=P, out_s=None, M=4, N=8, K=128, epi=0, dt=0)
+        a.update(kw)
+        return L.fw_gemm_e4m3_block_status(*a.values(), status, None)
+    assert call(M=0) == 0 and call(M=0, status=P) == 0
+    assert call(A=None, status=P) == EINVAL and call(K=0, status=P) == ESHAPE and call(out=P + 8, status=P) == EALIGN
+    assert call(status=P + 2) == EALIGN
+
+
+def test_every_wait_of_the_products_has_a_status():
+    for name in ("gemm_block.cu", "gemm_block_wide.cu"):
+        waits = re.findall(r"\b(?:wait_on(?:<true>)?|mbar_wait)\(([^;{]*)", source(name))
+        assert len(waits) >= 6
+        for w in waits:
+            assert re.search(r"a\.status,\s+DEV_TIMEOUT_", w), (name, w)
