@@ -294,15 +294,17 @@ __global__ void __launch_bounds__(W * 32, norm_warps(VEC, NB) / W) norm_gate_res
     const int c = c0 + b * b8::BLK;
     if (a.out_s) {
       const int blk = b0 + b;
-      if (blk * b8::BLK < Dp) {   // zeros behind D: every parameter reads as zero there
+      if (blk * b8::BLK < Dp) {
+        // Behind D every parameter reads as zero and so is the value, or it is NaN where the row's norm is; neither has
+        // a say in the exponent, and the codes there are zero.
         uint32_t eb;
         const uint32_t code = b8::encode_block(x[b], eb);
         uint8_t* o = static_cast<uint8_t*>(a.out) + (size_t)row * Dp + c;
         if (VEC) {
-          *reinterpret_cast<uint32_t*>(o) = code;
+          *reinterpret_cast<uint32_t*>(o) = c < D ? code : 0u;   // D % 4 == 0
         } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[i * STEP] = (uint8_t)(code >> (8 * i));
+          for (int i = 0; i < 4; ++i) o[i * STEP] = c + i * STEP < D ? (uint8_t)(code >> (8 * i)) : 0;
         }
         if (lane == 0) a.out_s[((size_t)(blk / b8::GRP) * a.M + row) * b8::GRP + blk % b8::GRP] = (uint8_t)eb;
       }

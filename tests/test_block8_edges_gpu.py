@@ -1,8 +1,10 @@
 """Block-scaled e4m3 linears and the norms around them at their edges.  Tolerances as in test_block8_gpu.py."""
+import math
+
 import pytest
 import torch
 
-from test_block8_gpu import operands, rand, value  # noqa: F401
+from test_block8_gpu import is_nan_code, norm_ref, operands, rand, value
 
 from test_failure_gpu import DEV_TIMEOUT_TEST, LIMIT_NS, gemm_still_correct, run_selftest
 
@@ -56,3 +58,28 @@ def test_status_of_a_product(M, N, K, out):
     for bad in (status.long(), status.cpu(), status[:0], status[::2]):
         with pytest.raises(ValueError, match="status"):
             ops.gemm_e4m3_block(a8, sa, b8, sb, out=out, status=bad)
+
+
+# ---------------------------------------------------------------- norms
+@pytest.mark.parametrize("D", [100, 300, 1283, 1535, 1536, 2050])
+@pytest.mark.parametrize("post,pre", [("layer", "rms"), ("rms", "layer"), (None, "layer"), ("layer", None), (None, None)])
+def test_norm_of_rows_that_are_not_finite(D, post, pre):
+    """A NaN or an infinity stays in its row, and where the formula has it; codes behind D are zero in every row."""
+    from fastworld_b200 import ops
+    M = 9
+    resid, y = rand(M, D, seed=1, dtype=torch.float32), rand(M, D, seed=2)
+    resid[1, 3], resid[3, D - 1], y[5, 0], y[7, D - 2] = math.nan, math.inf, math.nan, -math.inf
+    odd = torch.zeros(M, dtype=torch.bool, device="cuda")
+    odd[1::2] = True
+    x, h = norm_ref(resid, y, post, None, None, None, 1, 1, pre, None, None, None, None, M, 1e-6)
+    work = resid.clone()
+    q, s = ops.norm_gate_resid_(work, y, post=post, pre=pre, out="e4m3")
+    assert torch.equal(work.isnan(), x.isnan()) and torch.equal(work.isinf(), x.isinf())
+    assert torch.equal(is_nan_code(q[:, :D]), ~h.isfinite())       # infinities are held as the NaN code too
+    assert not q[:, D:].any()
+    clean, cy = resid[~odd].clone(), y[~odd].clone()
+    cq, cs = ops.norm_gate_resid_(clean, cy, post=post, pre=pre, out="e4m3")
+    assert torch.equal(q[~odd], cq) and torch.equal(s[:, ~odd], cs) and torch.equal(work[~odd], clean)
+    work = resid.clone()
+    b = ops.norm_gate_resid_(work, y, post=post, pre=pre)
+    assert torch.equal(b.isnan(), h.isnan()) and torch.equal(b.isinf(), h.isinf())
