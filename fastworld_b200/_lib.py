@@ -17,7 +17,7 @@ FW_MAX_STEPS = 16
 KIND_WEIGHT, KIND_STATE, KIND_INPUT, KIND_OUTPUT, KIND_WORKSPACE, KIND_STATUS, KIND_DERIVED = range(7)
 DT_BF16, DT_F32, DT_I32, DT_U8, DT_F16 = range(5)
 NORM_NONE, NORM_LAYER, NORM_RMS = range(3)
-BLOCK_MAX_COLS, NORM_MAX_COLS = 1 << 24, 16384
+BLOCK_MAX_COLS, NORM_MAX_COLS = 1 << 24, 16384   # columns that fw_*_block and fw_norm_gate_resid take
 EPI_BF16, EPI_GELU_BF16, EPI_RESID_F32, EPI_F32, EPI_GELU_ERF_BF16 = range(5)
 
 
@@ -80,6 +80,18 @@ class FwLbConfig(ctypes.Structure):
                 ("sink_frames", ctypes.c_int), ("n_steps", ctypes.c_int), ("eps", ctypes.c_float),
                 ("timesteps", ctypes.c_float * 8), ("sig_x0", ctypes.c_double * 8), ("an_alpha", ctypes.c_float * 8),
                 ("an_sigma", ctypes.c_float * 8)]
+
+
+class _Int(ctypes.c_int):
+    """An int argument: ctypes by itself cuts a larger number to its low 32 bits."""
+
+    @classmethod
+    def from_param(cls, v):
+        if not isinstance(v, int):
+            return ctypes.c_int.from_param(v)
+        if -0x80000000 <= v <= 0x7fffffff:
+            return v
+        raise ValueError(f"{v} does not fit an int")
 
 
 _SIGS = {
@@ -178,7 +190,7 @@ def lib() -> ctypes.CDLL:
         L = ctypes.CDLL(LIB_PATH)
         for name, (res, args) in _SIGS.items():
             f = getattr(L, name)
-            f.restype, f.argtypes = res, args
+            f.restype, f.argtypes = res, [_Int if a is ctypes.c_int else a for a in args]
         _LIB = L
     return _LIB
 

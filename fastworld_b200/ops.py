@@ -170,8 +170,9 @@ def quant_e4m3_block(x: torch.Tensor):
     uint8.  Each row's 128 columns share the smallest power of two 2^e (e >= -127) with
     max|x| <= 448 * 2^e over the finite elements; NaN and infinities become the NaN code."""
     dtype, index, shape = _DTYPES.get(x.dtype), x.get_device(), x.shape
-    if dtype is None or index < 0 or len(shape) != 2 or shape[1] == 0 or not x.is_contiguous():
-        _refuse("x", x, "bf16, fp16 or fp32", index, "[M, K > 0]")
+    if (dtype is None or index < 0 or len(shape) != 2 or not 0 < shape[1] <= _lib.BLOCK_MAX_COLS
+            or not x.is_contiguous()):
+        _refuse("x", x, "bf16, fp16 or fp32", index, f"[M, 0 < K <= {_lib.BLOCK_MAX_COLS}]")
     M, K = shape
     q, s = _block_empty(M, K, x.device)
     _on(index, lib().fw_quant_e4m3_block, "quant_e4m3_block", x.data_ptr(), dtype, M, K, q.data_ptr(), s.data_ptr())
@@ -189,12 +190,13 @@ def gemm_e4m3_block(a8: torch.Tensor, sa: torch.Tensor, b8: torch.Tensor, sb: to
     if out not in BLOCK_OUTPUTS:
         raise ValueError(f"out: {out!r}, expected one of {sorted(BLOCK_OUTPUTS)}")
     u8, index, shape = torch.uint8, a8.get_device(), a8.shape
-    if index < 0 or len(shape) != 2 or shape[1] == 0 or shape[1] % 128 or not _is(a8, u8, index):
-        _refuse("a8", a8, u8, index, "[M, a positive multiple of 128]")
+    if (index < 0 or len(shape) != 2 or not 0 < shape[1] <= _lib.BLOCK_MAX_COLS or shape[1] % 128
+            or not _is(a8, u8, index)):
+        _refuse("a8", a8, u8, index, f"[M, a multiple of 128 from 128 to {_lib.BLOCK_MAX_COLS}]")
     M, K = shape
     shape = b8.shape
-    if len(shape) != 2 or shape[1] != K or not _is(b8, u8, index):
-        _refuse("b8", b8, u8, index, f"[N, {K}]")
+    if len(shape) != 2 or shape[0] > _lib.BLOCK_MAX_COLS or shape[1] != K or not _is(b8, u8, index):
+        _refuse("b8", b8, u8, index, f"[N <= {_lib.BLOCK_MAX_COLS}, {K}]")
     N, groups = shape[0], -(-K // 512)
     if sa.shape != (groups, M, 4) or not _is(sa, u8, index):
         _refuse("sa", sa, u8, index, [groups, M, 4])
@@ -243,8 +245,9 @@ def norm_gate_resid_(resid: torch.Tensor, y=None, post=None, post_w=None, post_b
     quant_e4m3_block, quantised from fp32) or None (h is not computed).  resid's memory may be y's as a whole
     (fp32), and otherwise overlaps no argument."""
     f32, b16, index, shape = torch.float32, torch.bfloat16, resid.get_device(), resid.shape
-    if index < 0 or len(shape) != 2 or shape[1] == 0 or resid.dtype is not f32 or not resid.is_contiguous():
-        _refuse("resid", resid, f32, index, "[M, D > 0]")
+    if (index < 0 or len(shape) != 2 or shape[1] == 0 or max(shape) > 0x7fffffff or resid.dtype is not f32
+            or not resid.is_contiguous()):
+        _refuse("resid", resid, f32, index, f"[M, 0 < D <= {_lib.NORM_MAX_COLS}], M below 2^31")
     M, D = shape
     if post not in NORMS or pre not in NORMS:
         raise ValueError(f"post, pre: {post!r}, {pre!r}, expected 'layer', 'rms' or None")

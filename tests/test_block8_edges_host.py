@@ -1,7 +1,11 @@
 """Block-scaled e4m3 linears and the norms around them: what can be held to without a GPU."""
+import ctypes
 import glob
 import os
 import re
+
+import pytest
+import torch
 
 from test_block8_host import EALIGN, EINVAL, ESHAPE, L, P  # noqa: F401
 
@@ -69,3 +73,49 @@ def test_every_wait_of_the_products_has_a_status():
         assert len(waits) >= 6
         for w in waits:
             assert re.search(r"a\.status,\s+DEV_TIMEOUT_", w), (name, w)
+
+
+# ---------------------------------------------------------------- sizes
+def test_sizes_past_32_bits_are_refused_not_cut(L):
+    """2^32 + n would reach the library as n."""
+    cut = (1 << 32) + 128
+    for call in (lambda: L.fw_quant_e4m3_block(P, 0, 0, cut, P, P, None),
+                 lambda: L.fw_quant_e4m3_block(P, 0, 1 << 32, 128, P, P, None),
+                 lambda: L.fw_gemm_e4m3_block(P, P, P, P, P, P, None, 0, 8, cut, 0, 0, None),
+                 lambda: L.fw_gemm_e4m3_block_status(P, P, P, P, P, P, None, 1 << 32, 8, 128, 0, 0, None, None),
+                 lambda: L.fw_gemm_bf16(None, P, P, P, 1, 8, cut, 0, 0, None),
+                 lambda: L.fw_quant_e4m3(None, 1, -cut, P, P, None)):
+        with pytest.raises(ctypes.ArgumentError, match="does not fit an int"):
+            call()
+    assert L.fw_quant_e4m3_block(P, 0, 0, 2 ** 31 - 1, P, P, None) == ESHAPE
+
+
+class Fake:
+    """A tensor's face without its memory: what the wrappers look at before a launch."""
+
+    def __init__(self, *shape, dtype=torch.float32):
+        self.shape, self.dtype, self.device = torch.Size(shape), dtype, "cuda:0"
+
+    def get_device(self):
+        return 0
+
+    def is_contiguous(self):
+        return True
+
+    def stride(self):
+        return (self.shape[-1], 1)
+
+
+def test_wrappers_refuse_sizes_that_the_kernels_do_not_take():
+    from fastworld_b200 import ops
+    u8, top = torch.uint8, 1 << 24
+    s = Fake(1, 1, 4, dtype=u8)
+    for name, call in (("x", lambda: ops.quant_e4m3_block(Fake(1, (1 << 32) + 128, dtype=torch.bfloat16))),
+                       ("x", lambda: ops.quant_e4m3_block(Fake(1, top + 1))),
+                       ("a8", lambda: ops.gemm_e4m3_block(Fake(1, (1 << 32) + 128, dtype=u8), s, s, s)),
+                       ("a8", lambda: ops.gemm_e4m3_block(Fake(1, top + 128, dtype=u8), s, s, s)),
+                       ("b8", lambda: ops.gemm_e4m3_block(Fake(1, 128, dtype=u8), s, Fake(top + 1, 128, dtype=u8), s)),
+                       ("resid", lambda: ops.norm_gate_resid_(Fake(1 << 31, 1))),
+                       ("resid", lambda: ops.norm_gate_resid_(Fake(1, (1 << 32) + 1)))):
+        with pytest.raises(ValueError, match=name + ": expected"):
+            call()
