@@ -254,8 +254,8 @@ def norm_gate_resid_(resid: torch.Tensor, y=None, post=None, post_w=None, post_b
     if out not in ("bf16", "e4m3", None):
         raise ValueError(f"out: {out!r}, expected 'bf16', 'e4m3' or None")
     rpf = (M or 1) if rows_per_frame is None else int(rows_per_frame)
-    if rpf <= 0:
-        raise ValueError(f"rows_per_frame: {rows_per_frame}")
+    if rpf <= 0 or rows_per_frame is not None and rpf != rows_per_frame:
+        raise ValueError(f"rows_per_frame: {rows_per_frame}, expected a positive whole number")
     frames = -(-M // rpf)
     if y is None:
         if out is None:

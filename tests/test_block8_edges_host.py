@@ -119,3 +119,11 @@ def test_wrappers_refuse_sizes_that_the_kernels_do_not_take():
                        ("resid", lambda: ops.norm_gate_resid_(Fake(1, (1 << 32) + 1)))):
         with pytest.raises(ValueError, match=name + ": expected"):
             call()
+
+
+def test_rows_per_frame_is_a_whole_number():
+    """2.5 rows are not 2."""
+    from fastworld_b200 import ops
+    for rows in (2.5, 0.5, -1, 0):
+        with pytest.raises(ValueError, match="rows_per_frame"):
+            ops.norm_gate_resid_(Fake(4, 128), rows_per_frame=rows)
