@@ -4,7 +4,8 @@ import math
 import pytest
 import torch
 
-from test_block8_gpu import is_nan_code, norm_ref, operands, rand, value
+from test_block8_gpu import (is_nan_code, norm64, norm_ref, operands, pow2, rand, test_gemm_epilogues as epilogues,
+                             test_norm_gate_resid as norms, value)
 
 from test_failure_gpu import DEV_TIMEOUT_TEST, LIMIT_NS, gemm_still_correct, run_selftest
 
@@ -60,7 +61,79 @@ def test_status_of_a_product(M, N, K, out):
             ops.gemm_e4m3_block(a8, sa, b8, sb, out=out, status=bad)
 
 
+# tiles of 64 and of 128 rows whose k-blocks a cluster shares; the pair kernel's rows of C that no 16-byte store can
+# address (4500 bf16: the time model is far from the border at 4680 rows)
+@pytest.mark.parametrize("M,N,K", [(300, 1000, 4096), (512, 1536, 4096), (513, 1535, 4000), (4680, 4500, 2000)])
+@pytest.mark.parametrize("epi", ["none", "gelu_tanh", "gelu_erf"])
+@pytest.mark.parametrize("out", ["bf16", "e4m3"])
+def test_split_and_wide_epilogues(M, N, K, epi, out):
+    epilogues(M, N, K, epi, out)
+
+
+def test_e4m3_result_past_32_bits():
+    """The last rows of codes of more than 2^31 bytes."""
+    from fastworld_b200 import ops
+    M, N, last = 1100001, 2048, slice(-300, None)
+    a8, sa, b8, sb = operands(M, N, 128)
+    q, s = ops.gemm_e4m3_block(a8, sa, b8, sb, out="e4m3")
+    q, s = q[last].contiguous(), s[:, last].contiguous()
+    va, vb = value(a8[last], sa[:, last]), value(b8, sb)
+    ref, tol = va @ vb.t(), 132 * 2.0 ** -24 * (va.abs() @ vb.abs().t())
+    unit = pow2(s.permute(1, 0, 2).reshape(300, -1).double() - 127).repeat_interleave(128, 1)
+    step = torch.maximum(ref.abs() * 2.0 ** -4, unit * 2.0 ** -10)
+    assert ((value(q, s) - ref).abs() <= step * (1 + 1e-6) + 1.07 * tol).all()
+
+
 # ---------------------------------------------------------------- norms
+# with test_norm_widths, every number of warps per row and of blocks per warp over rows aligned to four elements and not
+@pytest.mark.parametrize("D", [383, 511, 1283, 1535, 2816, 2948])
+@pytest.mark.parametrize("out", ["bf16", "e4m3"])
+def test_norm_more_widths(D, out):
+    norms(21, D, 8, "layer", "rms", torch.bfloat16, out)
+    norms(3, D, 1, "rms", "layer", torch.float32, out)
+
+
+@pytest.mark.parametrize("D", [5, 384, 1535, 1536, 5120, 16384])
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("eps", [1e-6, 1e-5, 1e-3])
+def test_norm_statistics_in_fp32(D, kind, eps):
+    """Rows whose mean square is about eps or far below, and a row of zeros, as the norm after a block (fp32 out) and as
+    the one before the next (bf16 out).
+
+    A row's sums are added up by lane (at most 2 * 8 + 1 terms in a chain), across a warp (5) and across at most 16
+    warps, each a rounding: 38 of 2^-24.  1 / D, its product and eps add 4, so the reciprocal root is off by (38 + 4) / 2
+    and its own 4 (two units in the last place), the product with it by 1: 26, rounded up to 32.  LayerNorm's mean is off by
+    the 38 + 2 of mean|v| and the subtraction by 1, against the root: 42 r mean|v|."""
+    from fastworld_b200 import ops
+    u = 2.0 ** -24
+    y = rand(24, D, seed=3, dtype=torch.float32) * torch.tensor([0.0, 1e-4, 1e-3, 3e-3, 1e-2, 1.0],
+                                                                device="cuda").repeat(4)[:, None]
+    y[12:] += 0.5 * y[12:].abs().amax(1, keepdim=True)      # means that are not small
+    ref = norm64(y.double(), kind, eps)
+    v = y.double() - (y.double().mean(1, keepdim=True) if kind == "layer" else 0)
+    r = 1 / torch.sqrt((v * v).mean(1, keepdim=True) + eps)
+    tol = 32 * u * ref.abs() + (42 * u * r * y.double().abs().mean(1, keepdim=True) if kind == "layer" else 0)
+    x = torch.zeros(24, D, device="cuda")
+    assert ops.norm_gate_resid_(x, y, post=kind, eps=eps, out=None) is None
+    assert ((x.double() - ref).abs() <= tol).all()
+    assert not x[::6].any()
+    h = ops.norm_gate_resid_(y, pre=kind, eps=eps)
+    assert ((h.double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 1.01 * tol).all()
+    assert not h[::6].any()
+
+
+@pytest.mark.parametrize("D", [384, 1535, 5120])
+def test_norm_of_the_residual_itself(D):
+    """y may be the residual's own memory."""
+    from fastworld_b200 import ops
+    x = rand(50, D, seed=1, dtype=torch.float32)
+    kw = dict(post="rms", post_w=rand(D, seed=2), resid_scale=0.5, branch_scale=2.0, pre="layer")
+    apart = x.clone()
+    ref = ops.norm_gate_resid_(apart, x.clone(), **kw)
+    h = ops.norm_gate_resid_(x, x, **kw)
+    assert torch.equal(h, ref) and torch.equal(x, apart)
+
+
 @pytest.mark.parametrize("D", [100, 300, 1283, 1535, 1536, 2050])
 @pytest.mark.parametrize("post,pre", [("layer", "rms"), ("rms", "layer"), (None, "layer"), ("layer", None), (None, None)])
 def test_norm_of_rows_that_are_not_finite(D, post, pre):

@@ -127,3 +127,34 @@ def test_rows_per_frame_is_a_whole_number():
     for rows in (2.5, 0.5, -1, 0):
         with pytest.raises(ValueError, match="rows_per_frame"):
             ops.norm_gate_resid_(Fake(4, 128), rows_per_frame=rows)
+
+
+def test_calls_go_to_the_tensors_device_and_its_stream(monkeypatch):
+    """Tensors of another device than the current one: that device is made the current one around the launch, and its
+    current stream taken."""
+    from fastworld_b200 import ops
+    current, log = [0], []
+
+    class device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.back, current[0] = current[0], self.index
+
+        def __exit__(self, *_):
+            current[0] = self.back
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 100 + i, raising=False)
+    monkeypatch.setattr(torch.cuda, "device", device)
+
+    def fn(a, stream):
+        log.append((a, stream, current[0]))
+        return 0
+    ops._on(1, fn, "f", "x")
+    ops._on(0, fn, "f", "y")
+    assert log == [("x", 101, 1), ("y", 100, 0)] and current == [0]
+    with pytest.raises(RuntimeError):
+        ops._on(1, lambda *_: EINVAL, "f")
+    assert current == [0]
