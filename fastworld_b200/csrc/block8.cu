@@ -136,14 +136,14 @@ __device__ __forceinline__ float row_sum(float v, float* slot, int warp, int lan
   return t;
 }
 
-// Normalises x in place: fp32 mean and, about it, fp32 mean square (two sums, no cancellation).  Pairs of
-// columns on the packed fp32 pipe: with few rows per SM in flight, instructions count as much as bytes.
 // From one of a lane's four columns of a block to the next: where a row's addresses are not aligned to
 // four elements, a lane takes every 32nd column, so that each of the warp's scalar accesses is contiguous
 // (2640 x 1535 14.0 us; scalar accesses of four adjacent columns 27.0).
 template <bool VEC>
 constexpr int column_step = VEC ? 1 : 32;
 
+// Normalises x in place: fp32 mean and, about it, fp32 mean square (two sums, no cancellation).  Pairs of
+// columns on the packed fp32 pipe: with few rows per SM in flight, instructions count as much as bytes.
 template <bool VEC, int W, int NB>
 __device__ __forceinline__ void norm_row(float2 (&x)[NB][2], int kind, float eps, int D, int c0, float* slots, int warp,
                                          int lane) {
@@ -330,8 +330,8 @@ __global__ void __launch_bounds__(W * 32, norm_warps(VEC, NB) / W) norm_gate_res
 // 768 columns 3 x 2 13.1, 4 x 2 14.6, 4 x 3 17.4; 1152 columns 3 x 3 18.4, 4 x 3 19.9; for 4680 rows: 2560 columns
 // 7 x 3 31.2, 8 x 3 34.1; 4096 columns 8 x 4 45.4, 11 x 3 49.9, 10 x 4 52.2; 6144 columns 16 x 3 72.8, 12 x 4 72.8 (but 24.9
 // and 30.8 for 1000 rows of 6143), 16 x 4 83.2.  Fewer blocks per warp make more warps wait for a row's sums: 1536
-// columns 4 x 3 11.1 for 2640 rows, 6 x 2 12.2, 12 x 1 16.1; 5120 columns 10 x 4 66.8 for 4680 rows, 20 x 2 105 (these
-// before the registers were set).
+// columns 4 x 3 11.2 for 2640 rows, 6 x 2 11.5, 12 x 1 17.1; 5120 columns 10 x 4 57.2 for 4680 rows, 14 x 3 63.5, 20 x 2
+// 65.2; rows that are not aligned: 1535 columns 13.1, 13.8 and 18.0; 4799 columns 74, 76 and 112.
 template <typename Y, bool VEC>
 int norm_launch(const NormArgs& a, cudaStream_t s) {
   const int nb = b8::blocks(a.D);

@@ -58,8 +58,8 @@ __device__ __forceinline__ void umma_mx8_block(uint32_t one, uint32_t d, uint32_
 #undef FW_MX8
 }
 // In both CTAs of a pair, 32 rows of 16 bytes (512 contiguous bytes of its shared memory) to four columns of its
-// Tensor Memory, the same in every lane quarter: lane l of column c gets word c of row l.  Runs in order with
-// the MMAs of the issuing lane.
+// Tensor Memory, the same in every lane quarter: lane l of column c gets word c of row l.  Issued by another warp than
+// the MMAs that use the words: a commit behind the copies tells that they are there, one behind the MMAs that they are used.
 __device__ __forceinline__ void tmem_copy_pair_if(uint32_t one, uint32_t taddr, uint32_t saddr) {
   // descriptor: 128 bytes between 8-row groups, version 1, no swizzle
   const uint64_t desc = (uint64_t)((saddr >> 4) & 0x3fffu) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
