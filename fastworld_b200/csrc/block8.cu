@@ -60,8 +60,9 @@ struct Four<__half, true, STEP> {
 // A warp takes one row's group of 512 columns: four blocks, four columns per lane and block, so
 // each load and each store of codes is contiguous over the warp and a block's maximum is one warp
 // reduction.  The eight warps of a CTA take eight neighbouring rows, whose words of exponents are one 32-byte
-// sector.  Many short CTAs keep HBM busiest: 2640 x 8960 bf16 in 12.9 us (5.5 TB/s); warps that took two,
-// three or six groups with the next one's loads in flight took 16.0, 16.2 and 17.3 us.
+// sector.  Many short CTAs keep HBM busiest: 2640 x 8960 bf16 in 13.5 us (5.3 TB/s), fp32 in 18.5 us
+// (6.4 TB/s); warps that took two, three or six groups of bf16 with the next one's loads in flight took 16.0, 16.2 and
+// 17.3 us.
 constexpr int QROWS = 8;
 
 template <typename T, bool VEC>
@@ -118,9 +119,9 @@ struct NormArgs {
 
 // One row per CTA of W warps; warp w holds blocks [w NB, w NB + NB) of 128 columns in
 // registers, four columns per lane and block.  HBM bounds it (12 bytes per element in bf16), but a row's bytes wait
-// behind up to four sums over the row, so many rows have to be in flight: 2640 x 1536 in 11.7 us (4.2 TB/s),
-// 6032 x 1536 in 22.4 us (5.0 TB/s), 4680 x 5120 in 56.4 us (5.1 TB/s).  Slower: CTAs that take several rows,
-// the next one's loads in flight (16.8 us at 2640 x 1536), and rows brought to a ring in shared memory by bulk copies
+// behind up to four sums over the row, so many rows have to be in flight: 2640 x 1536 in 11.1 us (4.4 TB/s),
+// 6032 x 1536 in 21.5 us (5.2 TB/s), 4680 x 5120 in 54.0 us (5.3 TB/s), to e4m3 58.0.  Slower: CTAs that take several
+// rows, the next one's loads in flight (16.8 us at 2640 x 1536), and rows brought to a ring in shared memory by bulk copies
 // with a warp or four per row (27 us): fewer warps per SM are left to work through the sums; mean and square in one
 // sum of three numbers, joined pairwise (13.4 us); and asking for later rows in L2 ahead of their CTAs (2640 rows
 // 11.7 -> 11.8, 4680 rows 56.3 -> 54.4 in bf16 but 59.5 -> 60.2 in e4m3).

@@ -59,7 +59,8 @@ __device__ __forceinline__ void umma_mx8_block(uint32_t one, uint32_t d, uint32_
 }
 // In both CTAs of a pair, 32 rows of 16 bytes (512 contiguous bytes of its shared memory) to four columns of its
 // Tensor Memory, the same in every lane quarter: lane l of column c gets word c of row l.  Issued by another warp than
-// the MMAs that use the words: a commit behind the copies tells that they are there, one behind the MMAs that they are used.
+// the MMAs that use the words: a commit behind the copies tells that they are there, one behind the MMAs that they are
+// used.
 __device__ __forceinline__ void tmem_copy_pair_if(uint32_t one, uint32_t taddr, uint32_t saddr) {
   // descriptor: 128 bytes between 8-row groups, version 1, no swizzle
   const uint64_t desc = (uint64_t)((saddr >> 4) & 0x3fffu) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
@@ -127,7 +128,8 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
 // (the hardware's tanh.approx, relative error 2^-11, would show in an fp32 result, and 1 + tanh cancels
 // for negative v); where the power overflows the reciprocal is 0, as it should be.  erf form by erfc,
 // which keeps its relative precision where 1 + erf cancels: a block of small negative results is scaled by
-// them.  It is called, not inlined: its code, once per value, would not fit the epilogue loops.
+// them.  It is called, not inlined: its code, once per value, would not fit the epilogue loops.  2640 x 8960 x 1536
+// takes 38.0 us with the first form and 111 with the second.
 __device__ __forceinline__ float rcp_approx(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -28,8 +28,8 @@ namespace {
 // every splits-th row, adds the partials of all ranks in rank order (the same sum on every run) and writes it.
 //
 // What bounds it: with a few rows the weights' bytes behind about 4 us of launch, first loads and result
-// (1 x 1536 x 1536 4.8 us; 1 x 5120 x 13824, 71 MB, 15.4 us or 4.6 TB/s); with a few hundred rows the chain of
-// k-blocks of a CTA, 0.5 us each, which the split shortens for a join of 2.7 us (of 12.3 us at 512 x 1536 x 4096).
+// (1 x 1536 x 1536 4.4 us; 1 x 5120 x 13824, 71 MB, 16.0 us or 4.4 TB/s); with a few hundred rows the chain of
+// k-blocks of a CTA, 0.5 us each, which the split shortens for a join of 2.7 us (of 11.4 us at 512 x 1536 x 4096).
 namespace nk {
 constexpr int THREADS = 192, MAX_SPLITS = 8;
 template <int BN>
@@ -337,20 +337,21 @@ int launch_nk(const void* A8, const void* B8, const BlockGemmArgs& a, cudaStream
   }
 }
 
-// Which kernel, tile and split: the least of a time model (us) whose constants were fitted to measured times
-// (small tiles: 70 sizes of 1 to 4000 rows, 30 to 13824 columns, 60 to 8960 of K; between the two kernels: 37
-// sizes, where its choice is the faster one but for two, 4 and 7 % off).  Small tiles: launch, then the busiest SM's
-// operand bytes, or the latency of a CTA's chain of k-blocks, or HBM, then the exposed epilogue and the join of a
-// split; wide kernel: waves of 256 x 256 tiles, more for rows that no TMA store can address.
+// Which kernel, tile and split: the least of a time model (us) whose constants were fitted to measured times (small
+// tiles: 70 sizes of 1 to 4000 rows, 30 to 13824 columns, 60 to 8960 of K; between the two kernels: 37 sizes).  Of 52
+// sizes near the border measured since, nine went to the slower kernel by more than 2 %, most of them to small tiles
+// with a short K and an e4m3 or fp32 result (3250 x 1742 x 489 to e4m3 18.1 us, 9.9 wide). Small tiles: launch, then
+// the busiest SM's operand bytes, or the latency of a CTA's chain of k-blocks, or HBM, then the exposed epilogue and
+// the join of a split; wide kernel: waves of 256 x 256 tiles, more for rows that no TMA store can address.
 // Both sides, measured (us):
-//   small tiles   880 x 1536 x 8960   20.4 (split 3 ways; 30.9 unsplit)   25.5 wide
-//                 512 x 1536 x 13824  19.1                                36.5 wide
-//                 1001 x 777 x 1283    7.5                                10.7 wide
-//                 512 x 1536 x 4096   12.3 (split 5 ways; 16.2 unsplit)   17.9 wide
-//   wide         2640 x 1536 x 1536   9.9 small tiles                     9.5 wide
-//                 512 x 13824 x 5120  44.6                                33.9
-//                6032 x 1536 x 1536   19.7                                14.4
-//   a split         1 x 1536 x 1536    4.8 split 6 ways, 6.2 unsplit; 1 x 9216 x 1536 7.0 split 4 ways, 6.8 unsplit
+//   small tiles   880 x 1536 x 8960   18.7 (split 3 ways; 30.9 unsplit)   27.7 wide
+//                 512 x 1536 x 13824  18.5                                38.2 wide
+//                 1001 x 777 x 1283    7.6                                11.6 wide
+//                 512 x 1536 x 4096   11.4 (split 5 ways; 16.2 unsplit)   15.5 wide
+//   wide         2640 x 1536 x 1536   10.2 small tiles                    10.6 wide (the border)
+//                 512 x 13824 x 5120  45.6                                35.6
+//                6032 x 1536 x 1536   20.1                                15.8
+//   a split         1 x 1536 x 1536    4.4 split 6 ways, 6.2 unsplit; 1 x 9216 x 1536 7.0 split 4 ways, 6.8 unsplit
 // A split's CTAs fill at most 9/10 of two per SM: clusters do not fit every SM of a GPC, and what is left over
 // waits for whole tiles to end (512 x 1536 x 4096 on 64-row tiles split 3 ways, 288 CTAs: 18.6 us).
 struct Plan {

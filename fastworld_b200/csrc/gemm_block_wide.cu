@@ -19,12 +19,15 @@
 // What bounds it: the tensor core needs 2048 cycles for four k-blocks of 256 x 256 x 128, and their issue takes
 // 2240 (270 cycles for a block's four MMAs, 100 for its wait, 60 for its commit), 0.30 us a block; with all pairs
 // loading 0.36 us, 13 TB/s out of L2.  A call adds 4 us (first tile, last epilogue), a tile change 0.4 us.  2640 rows,
-// bf16 result: 4608 x 1536 18.2 us (2.05 PFLOP/s), 8960 x 1536 32.6 (2.2), 1536 x 8960 29.3 (2.5); 4680 x 13824 x 5120
-// 233 us (2.8), and 271 us when it repeats for seconds at the power limit.
-// Tried: tiles of 240 columns whose accumulators do not overlap (18.5 -> 20.7 us, 237 -> 260), four stages (240 ->
-// 245), a store wait and an exit barrier without release (18.5 -> 18.2; but then arrivals at a CTA that has left
-// are excluded by timing only); halves of 128 columns for a last wave that leaves pairs idle (issue takes as long
-// for a half: 880 x 1536 x 8960 26.6 -> 27.4); the next wait tried before a block's MMAs (30.1 -> 31.0).
+// bf16 result and bias, bursts of a millisecond at 1965 MHz: 4608 x 1536 19.7 us (1.9 PFLOP/s), 8960 x 1536 36.4 (2.0),
+// 1536 x 8960 31.8 (2.3); 4680 x 13824 x 5120 242 us (2.7), and 279 us when it repeats for seconds at the power limit
+// (1.30 GHz).  GELU in the tanh form hides behind the MMAs (8960 x 1536 38.0 us), in the erf form it does not (111 us:
+// an erfcf call for each value, where a tile's 12 k-blocks take 4 us).
+// Tried (before the exponents of the odd CTA were announced by a warp of their own with a release at cluster scope):
+// tiles of 240 columns whose accumulators do not overlap (18.5 -> 20.7 us, 237 -> 260), four stages (240 -> 245), a
+// store wait and an exit barrier without release (18.5 -> 18.2; but then arrivals at a CTA that has left are excluded
+// by timing only); halves of 128 columns for a last wave that leaves pairs idle (issue takes as long for a half: 880 x
+// 1536 x 8960 26.6 -> 27.4); the next wait tried before a block's MMAs (30.1 -> 31.0).
 #include "fw_gemm_block.cuh"
 
 namespace fw {
@@ -238,8 +241,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide::THREADS, 1)
       mbar_wait(drain + 1, 0, &no_abort, a.status, DEV_TIMEOUT_DRAIN);
     } else if (lane == 0) {
       // This CTA's groups announced to the even CTA's copier.  The release at cluster scope that its scales need
-      // waits for all that the thread has in flight: 0.6-1 us a group for warp 2 with the next group's loads
-      // (2640 x 8960 x 1536 with GELU to e4m3 40.3 us instead of 34.9), little for a thread that loads nothing.
+      // waits for all that the thread has in flight: by warp 2 itself, with the next group's loads, 1536 x 8960 took
+      // 33.4 us instead of 31.6 (two such warps, a group each in turn: no difference).
       const uint32_t sf_full0 = mapa_cluster(sf_full, 0);
       for (uint32_t grp = 0; grp < groups; ++grp) {
         const uint32_t slot = grp % SF_RING;
