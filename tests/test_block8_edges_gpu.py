@@ -156,3 +156,49 @@ def test_norm_of_rows_that_are_not_finite(D, post, pre):
     work = resid.clone()
     b = ops.norm_gate_resid_(work, y, post=post, pre=pre)
     assert torch.equal(b.isnan(), h.isnan()) and torch.equal(b.isinf(), h.isinf())
+
+
+# ---------------------------------------------------------------- long and wide ones, and the feed-forward pair
+def test_longest_sum():
+    """2^24 columns of ones: every partial sum is a whole number that fp32 holds."""
+    from fastworld_b200 import ops
+    K = 1 << 24
+    a8, sa = ops.quant_e4m3_block(torch.ones(2, K, device="cuda", dtype=torch.bfloat16))
+    b8, sb = ops.quant_e4m3_block(torch.ones(3, K, device="cuda", dtype=torch.bfloat16))
+    assert (ops.gemm_e4m3_block(a8, sa, b8, sb, out="f32") == K).all()
+
+
+def test_many_columns():
+    from fastworld_b200 import ops
+    M, N, K = 3, (1 << 20) + 5, 200
+    a8, sa, b8, sb = operands(M, N, K)
+    va, vb = value(a8, sa), value(b8, sb)
+    ref, mag = va @ vb.t(), va.abs() @ vb.abs().t()
+    out = ops.gemm_e4m3_block(a8, sa, b8, sb, out="f32")
+    assert ((out.double() - ref).abs() <= (K + 4) * 2.0 ** -24 * mag).all()
+
+
+def test_feed_forward_pair():
+    """The pair's result is the product of the codes between, which are right one by one: a hidden value on the other
+    side of a rounding border is a step of the format, and all that a plain form's result may differ by.  Alternating
+    inputs give each its own result, the same bits every time."""
+    from fastworld_b200 import ops
+    M, D, F = 2640, 1536, 8960
+    epilogues(M, F, D, "gelu_tanh", "e4m3")
+    up, down = operands(4, F, D, seed=21)[2:], operands(4, D, F, seed=22)[2:]
+    b1, b2 = rand(F, seed=23, size=0.1), rand(D, seed=24, size=0.1)
+
+    def pair(x):
+        h8, sh = ops.gemm_e4m3_block(*x, *up, b1, epilogue="gelu_tanh", out="e4m3")
+        return h8, sh, ops.gemm_e4m3_block(h8, sh, *down, b2)
+    xs = [operands(M, 4, D, seed=25 + i)[:2] for i in range(2)]
+    first = [pair(x) for x in xs]
+    assert not torch.equal(first[0][2], first[1][2])
+    for _ in range(5):
+        for x, ref in zip(xs, first):
+            assert all(torch.equal(g, r) for g, r in zip(pair(x), ref))
+    for h8, sh, got in first:
+        vh, vd = value(h8, sh), value(*down)
+        ref = vh @ vd.t() + b2.double()
+        mag = vh.abs() @ vd.abs().t() + b2.double().abs()
+        assert ((got.double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 1.01 * (F + 4) * 2.0 ** -24 * mag).all()
